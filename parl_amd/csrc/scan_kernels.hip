@@ -16,6 +16,7 @@
 //     lane l owns time steps [l*K, l*K+K), loads are coalesced along T, and the affine
 //     recurrence acc_t = d_t + a_t*acc_{t+1} is solved with a 6-step wavefront-shuffle suffix
 //     scan over (a, d) pairs; neighbours' V_{t+1} / vs_{t+1} come from one more shuffle.
+#include <atomic>
 #include <cstdlib>
 #include "common.hpp"
 #include <math.h>
@@ -781,17 +782,19 @@ __global__ __launch_bounds__(256) void discount_cumsum_kernel(
 // per-thread error flag used by the logits kernels (bad action index)
 __device__ int g_action_err;
 
-// address of the device-side data-error word (bad action / minibatch index), resolved once per
-// process; shared with ppo_kernels.hip
+// address of the CURRENT device's data-error word (bad action / minibatch index, a row of logits with NaN), looked up once
+// per device (a __device__ variable has one address on each); shared with the other kernel files
 int* device_error_flag() {
-  static int* p = nullptr;
-  if (!p) {
-    int* q = nullptr;
-    if (check(hipGetSymbolAddress((void**)&q, HIP_SYMBOL(g_action_err))) != PARLHIP_OK)
-      return nullptr;
-    p = q;
-  }
-  return p;
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int*> cached[kMaxDevices];
+  int dev = 0;
+  if (check(hipGetDevice(&dev)) != PARLHIP_OK) return nullptr;
+  if (dev >= 0 && dev < kMaxDevices)
+    if (int* p = cached[dev].load(std::memory_order_acquire)) return p;
+  int* q = nullptr;
+  if (check(hipGetSymbolAddress((void**)&q, HIP_SYMBOL(g_action_err))) != PARLHIP_OK) return nullptr;
+  if (dev >= 0 && dev < kMaxDevices) cached[dev].store(q, std::memory_order_release);
+  return q;
 }
 
 }  // namespace parlhip
