@@ -36,6 +36,11 @@ extern "C" {
 
 typedef void* parlhip_stream_t;
 
+/* element types of the entries that take more than float32 */
+#define PARLHIP_F32 0
+#define PARLHIP_BF16 1
+#define PARLHIP_F16 2
+
 /* library version (major*10000 + minor*100 + patch) and error text */
 int parlhip_version(void);
 /* sha256[:16] over the sources the library was built from (csrc/srchash.py): build hygiene, lets a
@@ -612,6 +617,64 @@ int parlhip_clip_adam_f32(int n_tensors, float* const* params, float* const* gra
                           float* const* exp_avg_sq, float* const* steps, const int64_t* numel, const float* lr,
                           double beta1, double beta2, double eps, double max_norm, float* workspace, float* norm_out,
                           parlhip_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Policies over large action sets: draw from logits, log-probability with gradient, global gradient norm.
+ * Device pointers must belong to the CURRENT device; `stream` too.
+ * ------------------------------------------------------------------------------------ */
+/* Draws one action per row of logits [B,A] (dtype PARLHIP_F32 / BF16 / F16, rows row_stride >= A elements apart, elements of
+ * a row adjacent) with the row's uniform (float64 in [0,1); anything else is clamped into it).  With x a row, m its maximum:
+ *   w_i = exp((x_i - m) / temperature), a weight under 2^-42 counts as 0; -inf marks an action that may not be taken
+ *   in the order (x descending, index ascending) the longest prefix is kept with position < top_k, mass before the
+ *   action < top_p * mass of the first top_k, and w_i >= min_p; the first action is always kept
+ *   actions[b] = the first index whose kept mass up to and with it exceeds uniform * kept mass
+ *   log_probs[b] = log softmax(x / temperature)[action], of the WHOLE row (parlhip_logits_log_prob gives the same)
+ * temperature 0: the largest logit, the lowest index among equals, log_prob 0.  top_k <= 0 or >= A, top_p >= 1, min_p 0: that
+ * filter is off.  Each setting is one value for all rows or, where the pointer is not NULL, float32 / int32 [B] on the
+ * device; there what lies outside a setting's range counts as its nearest end, a NaN as the narrowest choice.
+ * A row whose every logit is -inf gives action -1 and log_prob 0.  A row with a NaN or +inf gives action -1 and log_prob NaN
+ * and raises the data-error flag (parlhip_consume_device_errors); the other rows are not touched by it.
+ * Sums are integers (multiples of 2^-42 of the row's largest weight or finer), so the draw does not depend on how
+ * the work is split.  A <= 2^20 (else PARLHIP_ENOSUP).  workspace: parlhip_logits_sample_workspace_bytes(B, A) bytes,
+ * 8-byte aligned (may be NULL when that is 0).                                                                     */
+size_t parlhip_logits_sample_workspace_bytes(int64_t B, int64_t A);
+int parlhip_logits_sample(const void* logits, int dtype, int64_t row_stride, const double* uniforms,
+                          const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                          float temperature_all, int32_t top_k_all, float top_p_all, float min_p_all, int64_t* actions,
+                          float* log_probs, int64_t B, int64_t A, void* workspace, size_t workspace_bytes,
+                          parlhip_stream_t stream);
+/* Categorical(logits / temperature).log_prob(actions) and .entropy() (parl/algorithms/torch/ppo.py:104-121) of N rows of A
+ * logits (types and strides as above); actions int64 [N].  log_probs, entropies float32 [N]; stats float32 [N,2]
+ * (8-byte aligned, may be NULL): what the backward pass needs, the row's maximum and its sum of exp((x - max) / T).
+ * Action -1 marks a row that is no decision (padding): 0, 0, and a zero gradient; so does a row whose every logit is -inf.
+ * Another index outside [0,A) is clamped and raises the data-error flag.  A row with a NaN or +inf gives NaN.  float32 sums.
+ * workspace: parlhip_logits_log_prob_workspace_bytes(N, A) bytes (few long rows are split), 4-byte aligned.            */
+size_t parlhip_logits_log_prob_workspace_bytes(int64_t N, int64_t A);
+int parlhip_logits_log_prob(const void* logits, int dtype, int64_t row_stride, const int64_t* actions, float* log_probs,
+                            float* entropies, float* stats, int64_t N, int64_t A, float temperature, void* workspace,
+                            size_t workspace_bytes, parlhip_stream_t stream);
+/* The gradient: grad_logits [N,A] (contiguous, dtype of logits) = grad_log_probs * d log_prob + grad_entropies * d entropy,
+ * with the forward pass's stats and entropies; grad_log_probs / grad_entropies float32 [N], NULL counts as zeros.    */
+int parlhip_logits_log_prob_backward(const void* logits, int dtype, int64_t row_stride, const int64_t* actions,
+                                     const float* stats, const float* entropies, const float* grad_log_probs,
+                                     const float* grad_entropies, void* grad_logits, int64_t N, int64_t A,
+                                     float temperature, parlhip_stream_t stream);
+/* The global norm of n_tensors tensors, sqrt(sum of squares of all elements), -> norm_out float32 [1] (device).  HOST arrays:
+ * grads = device pointers (dense memory, numel[i] elements of types[i]), numel, types.  Any number of tensors; empty ones
+ * are skipped.  Squares and sums in float64, added in one fixed order (deterministic).  No host synchronisation;
+ * capturable: the host arrays are read during the call only.  workspace: parlhip_grad_norm_workspace_bytes(...)
+ * bytes, 8-byte aligned, for both entries.                                                                          */
+size_t parlhip_grad_norm_workspace_bytes(int n_tensors, const int64_t* numel);
+int parlhip_grad_norm(int n_tensors, const void* const* grads, const int64_t* numel, const int32_t* types,
+                      void* workspace, size_t workspace_bytes, float* norm_out, parlhip_stream_t stream);
+/* torch.nn.utils.clip_grad_norm_ (parl/algorithms/torch/a2c.py:76-78): every gradient times
+ * min(1, max_norm / (norm + 1e-6)), in place (outs and out_types NULL; nothing is written while the norm is under the bound)
+ * or into outs (device pointers, out_types may differ from types; outs[i] == grads[i] with one type is in place).
+ * norm_out = the norm before.  A NaN norm makes every gradient NaN.  PARLHIP_EINVAL where something written overlaps
+ * anything else that is read or written (a tensor given twice).  max_norm >= 0.                                       */
+int parlhip_clip_grad_norm(int n_tensors, const void* const* grads, void* const* outs, const int64_t* numel,
+                           const int32_t* types, const int32_t* out_types, double max_norm, void* workspace,
+                           size_t workspace_bytes, float* norm_out, parlhip_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -120,6 +120,15 @@ SIGNATURES = {
     'parlhip_vecnorm_reward_f64': (_i, [_p] * 8 + [_i, _d, _d, _d, _p]),
     'parlhip_ppo_sample_batch_f32': (_i, [_p] * 13 + [_i64, _i64, _i, _i, _p]),
     'parlhip_episode_stats_accum_f64': (_i, [_p, _p, _i, _p, _p]),
+    'parlhip_logits_sample_workspace_bytes': (_sz, [_i64, _i64]),
+    'parlhip_logits_sample':
+    (_i, [_p, _i, _i64] + [_p] * 5 + [_f, ctypes.c_int32, _f, _f, _p, _p, _i64, _i64, _p, _sz, _p]),
+    'parlhip_logits_log_prob_workspace_bytes': (_sz, [_i64, _i64]),
+    'parlhip_logits_log_prob': (_i, [_p, _i, _i64] + [_p] * 4 + [_i64, _i64, _f, _p, _sz, _p]),
+    'parlhip_logits_log_prob_backward': (_i, [_p, _i, _i64] + [_p] * 6 + [_i64, _i64, _f, _p]),
+    'parlhip_grad_norm_workspace_bytes': (_sz, [_i, _p]),
+    'parlhip_grad_norm': (_i, [_i, _p, _p, _p, _p, _sz, _p, _p]),
+    'parlhip_clip_grad_norm': (_i, [_i] + [_p] * 5 + [_d, _p, _sz, _p, _p]),
 }
 
 

@@ -1,0 +1,107 @@
+"""The C entries of the operators over logits and of the gradient norm refuse what they cannot do before they touch the device, and
+the Python entries refuse host tensors.  CPU only."""
+import ctypes
+
+import pytest
+import torch
+
+INVALID, NOSUP, NOMEM = -1, -3, -4
+
+
+@pytest.fixture(scope='module')
+def lib():
+    from parl_amd import _native
+    return _native.lib()
+
+
+def _sample(lib, logits=16, dtype=0, stride=8, u=16, t=None, k=None, p=None, mp=None, ta=1.0, ka=0, pa=1.0, ma=0.0, a=16, lp=16,
+            B=2, A=8, ws=16, wsb=1 << 40):
+    return lib.parlhip_logits_sample(logits, dtype, stride, u, t, k, p, mp, ta, ka, pa, ma, a, lp, B, A, ws, wsb, None)
+
+
+def test_sample_arguments(lib):
+    nan, inf = float('nan'), float('inf')
+    for kw in (dict(logits=None), dict(u=None), dict(a=None), dict(lp=None), dict(B=-1), dict(A=0), dict(stride=7), dict(ta=-1.0),
+               dict(ta=nan), dict(ta=inf), dict(pa=-0.5), dict(pa=nan), dict(ma=-0.5), dict(ma=2.0), dict(ma=nan),
+               dict(logits=18), dict(logits=17, dtype=1)):
+        assert _sample(lib, **kw) == INVALID, kw
+    assert _sample(lib, dtype=3) == NOSUP and _sample(lib, dtype=-1) == NOSUP
+    assert _sample(lib, A=(1 << 20) + 1, stride=1 << 21) == NOSUP
+    assert _sample(lib, B=1 << 40) == NOSUP
+    assert _sample(lib, B=0, logits=None, u=None, a=None, lp=None) == 0
+
+
+def test_log_prob_arguments(lib):
+    def f(x=16, dtype=0, stride=8, a=16, lp=16, h=16, st=16, N=2, A=8, T=1.0, ws=16, wsb=1 << 40):
+        return lib.parlhip_logits_log_prob(x, dtype, stride, a, lp, h, st, N, A, T, ws, wsb, None)
+
+    def b(x=16, dtype=0, stride=8, a=16, st=16, h=16, gl=16, gh=16, g=16, N=2, A=8, T=1.0):
+        return lib.parlhip_logits_log_prob_backward(x, dtype, stride, a, st, h, gl, gh, g, N, A, T, None)
+
+    nan, inf = float('nan'), float('inf')
+    for kw in (dict(x=None), dict(a=None), dict(N=-1), dict(A=0), dict(stride=7), dict(T=0.0), dict(T=-1.0), dict(T=nan),
+               dict(T=inf), dict(T=1e-39), dict(x=18), dict(x=17, dtype=2), dict(st=20)):
+        assert f(**kw) == INVALID, kw
+        assert b(**kw) == INVALID, kw
+    assert f(lp=None) == INVALID and f(h=None) == INVALID
+    assert b(st=None) == INVALID and b(h=None) == INVALID and b(g=None) == INVALID and b(g=18) == INVALID
+    assert f(dtype=7) == NOSUP and b(dtype=7) == NOSUP
+    assert f(N=1 << 39, A=1000, stride=1000) == NOSUP
+    assert f(N=0, x=None, a=None, lp=None, h=None) == 0 and b(N=0, x=None, a=None, st=None, h=None, g=None) == 0
+    need = lib.parlhip_logits_log_prob_workspace_bytes(1, 131072)
+    assert need > 0
+    assert f(N=1, A=131072, stride=131072, wsb=need - 1) == NOMEM
+    assert f(N=1, A=131072, stride=131072, ws=None) == INVALID
+    assert lib.parlhip_logits_log_prob_workspace_bytes(100000, 131072) == 0
+    assert lib.parlhip_logits_log_prob_workspace_bytes(5, 6) == 0
+
+
+def test_grad_norm_arguments(lib):
+    def arr(t, *v):
+        return (t * len(v))(*v)
+
+    P, I, T = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+    at, n, ty = arr(P, 4096, 8192), arr(I, 100, 200), arr(T, 0, 1)
+    assert lib.parlhip_grad_norm_workspace_bytes(2, n) == 16
+    assert lib.parlhip_grad_norm_workspace_bytes(2, arr(I, 0, 0)) == 8
+    assert lib.parlhip_grad_norm_workspace_bytes(2, arr(I, -1, 5)) == 0
+    assert lib.parlhip_grad_norm(-1, at, n, ty, 16, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, None, n, ty, 16, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, at, None, ty, 16, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, at, n, None, 16, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, at, n, ty, None, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, at, n, ty, 20, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, at, n, ty, 16, 1 << 30, None, None) == INVALID
+    assert lib.parlhip_grad_norm(2, at, n, ty, 16, 15, 16, None) == NOMEM
+    assert lib.parlhip_grad_norm(2, at, n, arr(T, 0, 3), 16, 1 << 30, 16, None) == NOSUP
+    assert lib.parlhip_grad_norm(2, at, arr(I, -1, 2), ty, 16, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, arr(P, None, 8192), n, ty, 16, 1 << 30, 16, None) == INVALID
+    assert lib.parlhip_grad_norm(2, arr(P, 4098, 8192), n, ty, 16, 1 << 30, 16, None) == INVALID
+
+    def c(at=at, out=None, n=n, ty=ty, oty=None, m=1.0):
+        return lib.parlhip_clip_grad_norm(2, at, out, n, ty, oty, m, 16, 1 << 30, 16, None)
+
+    assert c(m=-1.0) == INVALID and c(m=float('nan')) == INVALID
+    assert c(at=arr(P, 4096, 4096)) == INVALID and c(at=arr(P, 4096, 4096 + 396)) == INVALID      # the same memory twice
+    assert c(out=arr(P, 65536, 70000)) == INVALID and c(oty=ty) == INVALID
+    assert c(out=arr(P, 65536, None), oty=ty) == INVALID and c(out=arr(P, 65537, 70000), oty=ty) == INVALID
+    assert c(out=arr(P, 65536, 65600), oty=ty) == INVALID                                           # outputs overlap
+    assert c(out=arr(P, 8192, 70000), oty=ty) == INVALID                                            # ... another gradient
+    assert c(out=arr(P, 4100, 70000), oty=ty) == INVALID                                            # ... its own, shifted
+    assert c(out=arr(P, 4096, 8192), oty=arr(T, 1, 1)) == INVALID                                   # in place, another type
+
+
+def test_host_tensors_are_refused(lib):
+    from parl_amd import ops
+    from parl_amd._native import ParlHipError
+    x = torch.zeros(3, 5)
+    with pytest.raises(ParlHipError):
+        ops.logits_sample(x, torch.zeros(3, dtype=torch.float64))
+    with pytest.raises(ParlHipError):
+        ops.logits_log_prob(x, torch.zeros(3, dtype=torch.int64))
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(ParlHipError):
+        ops.clip_grad_norm_([p], 1.0)
+    with pytest.raises(ParlHipError):
+        ops.grad_norm([p.grad])
