@@ -161,6 +161,30 @@ def lib():
     return _lib
 
 
+_ops = None
+
+
+def torch_ops():
+    """Load (once) and return parl_amd._torch_ops, the entries of the library that are torch functions in C++
+    (csrc/torch_ops.cpp); raises if it is not built."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    handle = lib()
+    with _lock:
+        if _ops is None:
+            try:
+                from . import _torch_ops
+            except ImportError as e:
+                raise ImportError('parl_amd: _torch_ops.so is not built (%s). Build it with `python -c "import '
+                                  '__graft_entry__ as g; g.build()"` or `make -C parl_amd/csrc`. There is no fallback '
+                                  'path.' % e)
+            _torch_ops.bind(ParlHipError, {name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value
+                                           for name in SIGNATURES})
+            _ops = _torch_ops
+    return _ops
+
+
 def check(code, what):
     if code < 0:
         l = lib()

@@ -5,8 +5,6 @@ torch's current stream and returns torch tensors.  Nothing here computes on the 
 nothing falls back: a CPU tensor or a missing library raises ``ParlHipError``/``ImportError``.
 """
 
-import contextlib
-import numbers
 import os
 
 import torch
@@ -913,48 +911,6 @@ def ppo_sample_batch(obs, actions, logprobs, advantages, returns, values, idx):
     return (o_obs, o_act) + tuple(o4)
 
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # PARLHIP_F32 / BF16 / F16
-
-
-def _on_device_of(t):
-    """the kernels run on the tensors' device, on torch's current stream of it"""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
-
-
-def _check_logits(logits, name):
-    if logits.dtype not in _DTYPES:
-        raise N.ParlHipError('%s: logits must be float32, bfloat16 or float16, got %s' % (name, logits.dtype))
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise N.ParlHipError('%s: logits must be [..., A] with at least one action, got %s' % (name, tuple(logits.shape)))
-    if not logits.is_cuda:
-        raise N.ParlHipError('%s needs device (HIP) tensors; got a %s tensor. There is no CPU fallback.' %
-                             (name, logits.device))
-
-
-def _logit_rows(logits):
-    """(rows [N, A] with adjacent elements, dtype code, row stride): rows of a wider buffer (a padded action set) are read
-    in place, anything else is laid out first"""
-    A = logits.shape[-1]
-    x = logits.detach().reshape(logits.numel() // A, A)
-    stride = x.stride(0) if x.shape[0] > 1 else A
-    if stride < A or (A > 1 and x.stride(1) != 1):
-        x = x.contiguous()
-        stride = A
-    return x, _DTYPES[logits.dtype], stride
-
-
-def _per_row(t, dtype, like, what, name):
-    if t.dtype != dtype:
-        raise N.ParlHipError('%s: %s must be %s, got %s' % (name, what, dtype, t.dtype))
-    if t.device != like.device:
-        raise N.ParlHipError('%s: %s is on %s, logits on %s' % (name, what, t.device, like.device))
-    if tuple(t.shape) != tuple(like.shape[:-1]):
-        raise N.ParlHipError('%s: %s must have the shape %s, got %s' % (name, what, tuple(like.shape[:-1]), tuple(t.shape)))
-    return t.detach().contiguous()
-
-
 def logits_sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draw one action per row of logits [..., A] (float32 / bfloat16 / float16, A up to 2^20) with the given uniforms
     (float64 [...], in [0, 1)): np.random.choice(A, 1, p=softmax(logits)) (examples/IMPALA/atari_agent.py:38-40) with the
@@ -969,76 +925,7 @@ def logits_sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     log_probs are those of the WHOLE distribution softmax(logits / temperature), what logits_log_prob gives the learner
     for the same action (0 where the temperature is 0).  A row without a legal action gives action -1 and log_prob 0 (and
     logits_log_prob ignores action -1); a row with NaN or +inf gives -1, NaN and the flag of consume_device_errors()."""
-    name = 'logits_sample'
-    _check_logits(logits, name)
-    x, code, stride = _logit_rows(logits)
-    u = _per_row(uniforms, torch.float64, logits, 'uniforms', name)
-    keep, args, alls = [], [], []
-    for what, v, dtype, ok in (('temperature', temperature, torch.float32, lambda v: 0.0 <= v < float('inf')),
-                               ('top_k', top_k, torch.int32, lambda v: isinstance(v, numbers.Integral) and -2**31 <= v < 2**31),
-                               ('top_p', top_p, torch.float32, lambda v: v >= 0.0),
-                               ('min_p', min_p, torch.float32, lambda v: 0.0 <= v <= 1.0)):
-        if isinstance(v, torch.Tensor):
-            keep.append(_per_row(v, dtype, logits, what, name))
-            args.append(N.ptr(keep[-1]))
-            alls.append(0 if dtype == torch.int32 else 1.0)
-            continue
-        if not ok(v):
-            raise N.ParlHipError('%s: %s must be %s, got %r' % (name, what, {
-                'temperature': 'a finite number >= 0', 'top_k': 'a whole number of 32 bits', 'top_p': 'a number >= 0',
-                'min_p': 'a number in [0, 1]'}[what], v))
-        args.append(None)
-        alls.append(int(v) if dtype == torch.int32 else float(v))
-    rows, A = x.shape
-    with _on_device_of(x):
-        actions = torch.empty(logits.shape[:-1], dtype=torch.int64, device=x.device)
-        log_probs = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
-        wsb = N.lib().parlhip_logits_sample_workspace_bytes(rows, A)
-        ws = torch.empty(wsb // 8, dtype=torch.float64, device=x.device) if wsb else None
-        N.check(
-            N.lib().parlhip_logits_sample(x.data_ptr(), code, stride, N.ptr(u), *args, *alls, N.ptr(actions),
-                                          N.ptr(log_probs), rows, A, N.ptr(ws), wsb, N.stream_ptr()),
-            'parlhip_logits_sample')
-    return actions, log_probs
-
-
-class _LogitsLogProbFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, actions, temperature):
-        x, code, stride = _logit_rows(logits)
-        rows, A = x.shape
-        with _on_device_of(x):
-            log_probs = torch.empty(logits.shape[:-1], dtype=torch.float32, device=x.device)
-            entropies = torch.empty_like(log_probs)
-            stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device)
-            wsb = N.lib().parlhip_logits_log_prob_workspace_bytes(rows, A)
-            ws = torch.empty(wsb // 4, dtype=torch.float32, device=x.device) if wsb else None
-            N.check(
-                N.lib().parlhip_logits_log_prob(x.data_ptr(), code, stride, N.ptr(actions), N.ptr(log_probs),
-                                                N.ptr(entropies), N.ptr(stats), rows, A, temperature, N.ptr(ws), wsb,
-                                                N.stream_ptr()), 'parlhip_logits_log_prob')
-        ctx.save_for_backward(logits, actions, stats, entropies)
-        ctx.temperature = temperature
-        ctx.set_materialize_grads(False)
-        return log_probs, entropies
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_logp, g_ent):
-        if g_logp is None and g_ent is None:
-            return None, None, None
-        logits, actions, stats, entropies = ctx.saved_tensors
-        x, code, stride = _logit_rows(logits)
-        rows, A = x.shape
-        with _on_device_of(x):
-            g_logp, g_ent = [None if g is None else g.to(torch.float32).contiguous() for g in (g_logp, g_ent)]
-            grad = torch.empty(logits.shape, dtype=logits.dtype, device=x.device)
-            N.check(
-                N.lib().parlhip_logits_log_prob_backward(x.data_ptr(), code, stride, N.ptr(actions), N.ptr(stats),
-                                                         N.ptr(entropies), N.ptr(g_logp), N.ptr(g_ent), N.ptr(grad),
-                                                         rows, A, ctx.temperature, N.stream_ptr()),
-                'parlhip_logits_log_prob_backward')
-        return grad, None, None
+    return N.torch_ops().logits_sample(logits, uniforms, temperature, top_k, top_p, min_p)
 
 
 def logits_log_prob(logits, actions, temperature=1.0):
@@ -1050,66 +937,13 @@ def logits_log_prob(logits, actions, temperature=1.0):
     Action -1 marks a row that is no decision (padding behind a sequence's end): log_prob 0, entropy 0, zero gradient; so
     does a row whose every logit is -inf.  Another index outside [0, A) is clamped and raises the flag of
     consume_device_errors().  A row with NaN or +inf gives NaN; the other rows are not touched by it."""
-    name = 'logits_log_prob'
-    _check_logits(logits, name)
-    actions = _per_row(actions, torch.int64, logits, 'actions', name)
-    temperature = float(temperature)
-    if not 0.0 < temperature < float('inf'):
-        raise N.ParlHipError('%s: temperature must be a finite number > 0, got %r' % (name, temperature))
-    return _LogitsLogProbFn.apply(logits, actions, temperature)
-
-
-def _dense(t):
-    """whether the elements fill their memory, in whatever order of the axes"""
-    if t.is_contiguous():
-        return True
-    want = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
-        if stride != want:
-            return False
-        want *= size
-    return True
-
-
-def _norm_table(tensors, name):
-    """HOST arrays (addresses, sizes, type codes) of the tensors, which are on one device"""
-    import ctypes
-    dev = None
-    for t in tensors:
-        if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.dtype not in _DTYPES:
-            raise N.ParlHipError('%s: needs dense float32, bfloat16 or float16 tensors, got %s' %
-                                 (name, '%s %s' % (t.layout, t.dtype) if isinstance(t, torch.Tensor) else type(t)))
-        if not t.is_cuda or (dev is not None and t.device != dev):
-            raise N.ParlHipError('%s: the tensors must be on one HIP device, got %s%s' %
-                                 (name, t.device, '' if dev is None else ' and %s' % dev))
-        if not _dense(t):
-            raise N.ParlHipError('%s: a tensor of shape %s and strides %s does not fill its memory' %
-                                 (name, tuple(t.shape), t.stride()))
-        dev = t.device
-    n = len(tensors)
-    return dev, ((ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
-                 (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
-                 (ctypes.c_int32 * n)(*[_DTYPES[t.dtype] for t in tensors]))
-
-
-def _gradients(parameters):
-    ps = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    return [p.grad for p in ps if p.grad is not None]
+    return N.torch_ops().logits_log_prob(logits, actions, temperature)
 
 
 def grad_norm(tensors):
     """The global norm sqrt(sum of squares of all elements) of any number of tensors (float32 / bfloat16 / float16, mixed, on
     one device) as a float32 scalar tensor on the device (no synchronisation).  Sums in float64 in one fixed order."""
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    dev, (at, numel, types) = _norm_table(tensors, 'grad_norm')
-    norm = torch.empty((), dtype=torch.float32, device=dev or torch.device('cuda', torch.cuda.current_device()))
-    with _on_device_of(norm):
-        wsb = N.lib().parlhip_grad_norm_workspace_bytes(len(tensors), numel)
-        ws = torch.empty(wsb // 8, dtype=torch.float64, device=norm.device)
-        N.check(
-            N.lib().parlhip_grad_norm(len(tensors), at, numel, types, N.ptr(ws), wsb, N.ptr(norm), N.stream_ptr()),
-            'parlhip_grad_norm')
-    return norm
+    return N.torch_ops().grad_norm(tensors)
 
 
 def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False, out=None):
@@ -1121,35 +955,7 @@ def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False, out=None):
     out: a list of tensors, one for each parameter with a gradient, that receive the clipped gradients instead (of any
     of the three types, e.g. the float32 gradients of master weights); the .grad stay as they are.  A gradient
     given twice, or an `out` that overlaps another tensor of the call, is refused."""
-    name = 'clip_grad_norm_'
-    max_norm = float(max_norm)
-    if not max_norm >= 0.0:
-        raise N.ParlHipError('%s: max_norm must be >= 0, got %r' % (name, max_norm))
-    grads = _gradients(parameters)
-    dev, (at, numel, types) = _norm_table(grads, name)
-    o_at = o_types = None
-    if out is not None:
-        out = list(out)
-        if len(out) != len(grads):
-            raise N.ParlHipError('%s: out has %d tensors for %d gradients' % (name, len(out), len(grads)))
-        o_dev, (o_at, _, o_types) = _norm_table(out, name)
-        for g, o in zip(grads, out):
-            if o.device != g.device or o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise N.ParlHipError('%s: an out of shape %s, strides %s on %s for a gradient of shape %s, strides %s on %s' %
-                                     (name, tuple(o.shape), o.stride(), o.device, tuple(g.shape), g.stride(), g.device))
-    if error_if_nonfinite:
-        norm = grad_norm(grads)
-        if not bool(torch.isfinite(norm)):
-            raise RuntimeError('%s: the global norm of the gradients is %s; they are unchanged' % (name, float(norm)))
-    norm = torch.empty((), dtype=torch.float32, device=dev or torch.device('cuda', torch.cuda.current_device()))
-    with _on_device_of(norm):
-        wsb = N.lib().parlhip_grad_norm_workspace_bytes(len(grads), numel)
-        ws = torch.empty(max(wsb // 8, 1), dtype=torch.float64, device=norm.device)
-        N.check(
-            N.lib().parlhip_clip_grad_norm(len(grads), at, o_at, numel, types, o_types, max_norm, N.ptr(ws), wsb,
-                                           N.ptr(norm), N.stream_ptr()), 'parlhip_clip_grad_norm')
-    torch.autograd.graph.increment_version(out if out is not None else grads)   # written through raw pointers
-    return norm
+    return N.torch_ops().clip_grad_norm(parameters, max_norm, error_if_nonfinite, out)
 
 
 def consume_device_errors():
