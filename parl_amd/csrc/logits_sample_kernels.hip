@@ -12,12 +12,17 @@
 // kernel below draw the same action from the same row.  (Sums in float32 would move the draw of about one row in a
 // hundred over 131,072 actions: the border between two actions has to be right to far less than their weights.)
 //
-// No sort.  What top-k and top-p keep is "larger than a cut value, and the first few that equal it".  The cut is found by a
-// histogram of counts and masses over 256 classes of -log2 w, a scan of the classes, and the same again inside the class
-// that holds the border (on a list of its values in LDS, or on the row where a flat row puts more into one class than
-// the list takes) until a class is a single value.  Then one pass sums what is kept, segment by segment in index order, and
-// the segment that the draw falls into is scanned.  Three forms by size: lanes of a wave (A <= 64), a workgroup per row,
-// and three launches over parts of the row where the rows are few and long.
+// No sort.  Rows of at most 64 actions take lanes of a wave.  Longer rows:
+//   no filter   one pass: every wave sums the weights of 4 KB at a time relative to their own maximum; the sums are brought
+//               to the row's maximum, the piece that the draw falls into is found among them and scanned.
+//   filters     what they keep is "larger than a cut value, and the first few that equal it".  One pass for the maximum,
+//               one that adds masses (and counts, for top-k) into 256 classes of -log2 w, for each segment of the
+//               row; the class that holds the border is found by a scan and taken apart on a list of its
+//               values in LDS, by the same histogram over ever fewer bits (or on the row itself, where a flat row puts
+//               more values into one class than the list takes).  The classes above the border and the list give the
+//               kept mass of every segment, and the segment that the draw falls into is scanned.
+//   few rows    are cut into parts, one workgroup each, for the passes over the whole row; a workgroup per row joins
+//               what they leave in the workspace and goes on as above.
 #include "common.hpp"
 #include "logits_common.hpp"
 
@@ -26,7 +31,7 @@ namespace parlhip {
 constexpr int64_t kSampleMaxActions = (int64_t)1 << 20;
 constexpr double kFloorLog2 = -42.0;     // weights under 2^-42 are 0
 constexpr int kBins = 256;
-constexpr int kList = 4096;
+constexpr int kMaxParts = 64;       // of a row that several workgroups share
 
 struct SampleArgs {
   const double* uniforms;
@@ -68,8 +73,8 @@ __device__ __forceinline__ Row row_settings(const SampleArgs& q, int64_t row) {
   return r;
 }
 
-// whether the cut needs the histogram
-__device__ __forceinline__ bool needs_histogram(const Row& r) { return r.k > 1 || r.top_p < 1.f; }
+// whether anything but the maximum and the whole mass is asked for
+__device__ __forceinline__ bool filtered(const Row& r) { return !r.greedy && (r.k > 0 || r.top_p < 1.f || r.ymin > kFloorLog2); }
 
 // the order of values as unsigned integers; -0 is 0
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -83,23 +88,24 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // log2 of a weight; 0 at the maximum
 __device__ __forceinline__ double log2_weight(float x, float m, double c) { return ((double)x - (double)m) * c; }
 
-// 2^y in units of 2^-shift, rounded to nearest; y in [-42, 0], shift <= 51.  2^r = 1 + r q(r) on |r| <= 1/2 with q the
-// interpolation of (2^r - 1) / r at nine Chebyshev nodes: relative error 4e-14, and 2^0 is 1.  Adding 2^52 to a number below
-// it leaves its nearest integer in the low bits.
+// 2^y in units of 2^-shift, rounded to nearest, 0 where y < -42; y <= 0, shift <= 51.  2^r = 1 + r q(r) on |r| <= 1/2 with
+// q the interpolation of (2^r - 1) / r at eight Chebyshev nodes: relative error 2e-12, and 2^0 is 1.  Adding 2^52 to a
+// number below it leaves its nearest integer in the low bits.  No branch: the weights of a load are formed side by side.
+// Some 75 cycles of the vector unit for 64 weights; float64 runs at float32's rate here.
 __device__ __forceinline__ uint64_t weight_units(double y, int shift) {
   const double n = rint(y), r = y - n;
-  double p = 0x1.b63880a30e9ffp-24;
-  p = __builtin_fma(p, r, 0x1.63d136366db24p-20);
-  p = __builtin_fma(p, r, 0x1.ffcb9515a8016p-17);
-  p = __builtin_fma(p, r, 0x1.4308ac85aa947p-13);
-  p = __builtin_fma(p, r, 0x1.5d87fe86fe88ep-10);
-  p = __builtin_fma(p, r, 0x1.3b2ab7181b755p-7);
-  p = __builtin_fma(p, r, 0x1.c6b08d7047e52p-5);
-  p = __builtin_fma(p, r, 0x1.ebfbdff823cedp-3);
-  p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);
+  double p = 0x1.63b2d7971923fp-20;
+  p = __builtin_fma(p, r, 0x1.00c0e4e15189cp-16);
+  p = __builtin_fma(p, r, 0x1.4308c7183d6a2p-13);
+  p = __builtin_fma(p, r, 0x1.5d877598350dep-10);
+  p = __builtin_fma(p, r, 0x1.3b2ab70ad2565p-7);
+  p = __builtin_fma(p, r, 0x1.c6b08da70cce3p-5);
+  p = __builtin_fma(p, r, 0x1.ebfbdff82a734p-3);
+  p = __builtin_fma(p, r, 0x1.62e42fef9cc69p-1);
   p = __builtin_fma(p, r, 1.0);
-  const double v = __builtin_amdgcn_ldexp(p, (int)n + shift) + 0x1p52;
-  return (uint64_t)__double_as_longlong(v) & 0xfffffffffffffULL;
+  const double scale = __hiloint2double((int)((uint32_t)((int)n + shift + 1023) << 20), 0);   // 2^(n + shift)
+  const uint64_t bits = (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
+  return y >= kFloorLog2 ? bits & 0xfffffffffffffULL : 0;
 }
 
 // the class of a weight: 0 for the largest, 255 for those just above 2^-42
@@ -195,50 +201,87 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
 }
 
 // ------------------------------------------------------------------------------------------------------------------
-// A workgroup per row (or per part of a row).
+// Longer rows: a workgroup of NT threads for a row or a part of one.
+
+// f(v, i) for the vectors of [begin, end) of a row, by the threads tid < NT, four loads in flight: v are the V elements from
+// i on; what lies behind the end is -inf, which has no weight.  begin is a multiple of V.
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void for_each_vec(const T* __restrict__ x, int begin, int end, int tid, F&& f) {
+  constexpr int V = Vec16<T>::n;
+  int i = begin + tid * V;
+  for (; i + 3 * NT * V + V <= end; i += 4 * NT * V) {
+    Vec16<T> v[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) v[a].load(x + i + a * NT * V);
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      float g[V];
+      v[a].unpack(g);
+      f(g, i + a * NT * V);
+    }
+  }
+  for (; i < end; i += NT * V) {
+    float g[V];
+    if (i + V <= end) {
+      Vec16<T> v;
+      v.load(x + i);
+      v.unpack(g);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = i + j < end ? to_f32(x[i + j]) : -INFINITY;
+    }
+    f(g, i);
+  }
+}
+
+// the pieces of a row whose weights are summed relative to their own maximum: what a wave loads at a time
+template <typename T>
+__host__ __device__ constexpr int piece_length() { return 64 * 4 * 16 / (int)sizeof(T); }
+
+struct Pieces {          // of one row, in LDS or in the workspace
+  uint64_t* mass;
+  float* max;
+};
 
 template <typename T, int NT>
 struct RowWork {
   static constexpr int kWaves = NT / 64;
-  uint64_t mass[kBins];
+  static constexpr int kList = NT == 1024 ? 4096 : NT == 256 ? 2048 : 1024;
+  static constexpr int kPieces = NT == 1024 ? 1024 : NT == 256 ? 16 : 2;
+  union {
+    uint64_t wave_mass[kWaves][kBins];   // the histogram of each wave's segment
+    struct {
+      uint64_t mass[kPieces];
+      float max[kPieces];
+    } piece;
+  };
+  uint64_t mass[kBins];                  // of the row, or of the class that is being taken apart
   uint32_t count[kBins];
-  uint32_t list[kList];
-  uint64_t seg_mass[kWaves];
-  uint32_t seg_ties[kWaves];
+  uint32_t list[kList];                  // the values (keys) of a class and the segments that they are in
+  uint8_t list_seg[kList];
+  uint64_t seg_mass[kMaxParts];
+  uint32_t seg_ties[kMaxParts];
   uint64_t red64[kWaves];
   uint32_t red32[kWaves];
-  uint32_t lo, hi, n;                    // of the class under refinement
+  uint32_t lo, hi, n;                    // of the listed class
   int bin;                               // what the scan found
   uint64_t above_mass;
   uint32_t above_count;
   int found;
+  uint64_t found_target;
 };
 
-// f(value, index) for the elements [begin, end) of a row, spread over NT threads, four loads in flight; no order
-template <typename T, int NT, typename F>
-__device__ __forceinline__ void for_each(const T* __restrict__ x, int64_t begin, int64_t end, int tid, F&& f) {
-  constexpr int V = Vec16<T>::n;
-  int64_t i = begin + (int64_t)tid * V;
-  for (; i + (int64_t)(3 * NT) * V + V <= end; i += (int64_t)4 * NT * V) {
-    Vec16<T> v[4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a) v[a].load(x + i + (int64_t)a * NT * V);
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-      for (int j = 0; j < V; ++j) f(v[a].get(j));
-  }
-  for (; i < end; i += (int64_t)NT * V) {
-    if (i + V <= end) {
-      Vec16<T> v;
-      v.load(x + i);
-#pragma unroll
-      for (int j = 0; j < V; ++j) f(v.get(j));
-    } else {
-      for (int64_t j = i; j < end; ++j) f(to_f32(x[j]));
-    }
-  }
-}
+// a row, its settings, and the segments that its sums are kept by
+template <typename T>
+struct RowView {
+  const T* x;
+  int A;
+  float m;
+  Row r;
+  int shift;
+  int n_seg, seg_len;                    // segment s: [s * seg_len, ...); seg_len is a multiple of every vector
+  const uint64_t* seg_hist;              // [n_seg][kBins]
+};
 
 template <typename X, int NT>
 __device__ __forceinline__ X group_sum(X v, X* lds) {   // every thread gets the sum
@@ -255,51 +298,127 @@ __device__ __forceinline__ X group_sum(X v, X* lds) {   // every thread gets the
   return v;
 }
 
-// the maximum of [begin, end); bad: a NaN or +inf among them
-template <typename T, int NT>
-__device__ __forceinline__ float part_max(const T* __restrict__ x, int64_t begin, int64_t end, bool& bad, uint32_t* lds) {
-  float m = -INFINITY;
-  uint32_t b = 0;
-  for_each<T, NT>(x, begin, end, threadIdx.x, [&](float v) {
-    b |= !(v < INFINITY);
-    m = fmaxf(m, v);
-  });
+// the largest value over the group, and whether any thread saw a NaN or +inf
+template <int NT>
+__device__ __forceinline__ float group_max(float m, bool& bad, uint32_t* lds) {
   m = wave_max_f32(m);
-  b = __any(b) ? 1 : 0;
+  bad = __any(bad);
   if constexpr (NT > 64) {
-    const int w = threadIdx.x >> 6;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[w] = value_key(m) | 0;
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = bad ? 0xffffffffu : value_key(m);   // no value has that key
     __syncthreads();
     uint32_t k = lds[0];
 #pragma unroll
     for (int o = 1; o < NT / 64; ++o) k = lds[o] > k ? lds[o] : k;
+    bad = k == 0xffffffffu;
     m = key_value(k);
-    b = group_sum<uint32_t, NT>((threadIdx.x & 63) == 0 ? b : 0, lds);
   }
-  bad = b != 0;
   return m;
 }
 
-// counts and masses of the classes of [begin, end) -> w.count, w.mass (cleared here); returns this thread's mass
+// this thread's share of the maximum of [begin, end)
 template <typename T, int NT>
-__device__ __forceinline__ uint64_t part_histogram(const T* __restrict__ x, int64_t begin, int64_t end, float m, const Row& r,
-                                                   int shift, RowWork<T, NT>& w) {
-  for (int i = threadIdx.x; i < kBins; i += NT) { w.mass[i] = 0; w.count[i] = 0; }
-  __syncthreads();
-  uint64_t total = 0;
-  for_each<T, NT>(x, begin, end, threadIdx.x, [&](float v) {
-    const double y = log2_weight(v, m, r.c);
-    if (y >= kFloorLog2) {
-      const uint64_t u = weight_units(y, shift);
-      total += u;
-      const int b = weight_bin(y);
-      atomicAdd(&w.count[b], 1u);
-      atomicAdd((unsigned long long*)&w.mass[b], (unsigned long long)u);
+__device__ __forceinline__ float part_max(const T* __restrict__ x, int begin, int end, bool& bad) {
+  float m = -INFINITY;
+  bool b = false;
+  for_each_vec<T, NT>(x, begin, end, threadIdx.x, [&](const float (&v)[Vec16<T>::n], int) {
+#pragma unroll
+    for (int j = 0; j < Vec16<T>::n; ++j) {
+      b |= !(v[j] < INFINITY);
+      m = fmaxf(m, v[j]);
     }
   });
+  bad = b;
+  return m;
+}
+
+// The pieces [first, last) of a row, one after the other by each of the waves `wave` of `waves`: their maxima and their
+// masses relative to these.  bad: a NaN or +inf was seen.  -inf as a maximum: a piece without a legal action.
+template <typename T>
+__device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, double c, int shift, int first, int last, int wave,
+                                           int waves, const Pieces& out, bool& bad) {
+  constexpr int V = Vec16<T>::n, kLen = piece_length<T>();
+  const int lane = threadIdx.x & 63;
+  bad = false;
+  for (int p = first + wave; p < last; p += waves) {
+    const int base = p * kLen + lane * V;
+    float v[4][V];
+    if (p * kLen + kLen <= A) {
+      Vec16<T> raw[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) raw[a].load(x + base + a * 64 * V);
+#pragma unroll
+      for (int a = 0; a < 4; ++a) raw[a].unpack(v[a]);
+    } else {
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int i = base + a * 64 * V + j;
+          v[a][j] = i < A ? to_f32(x[i]) : -INFINITY;
+        }
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        bad |= !(v[a][j] < INFINITY);
+        m = fmaxf(m, v[a][j]);
+      }
+    m = wave_max_f32(m);
+    uint64_t mass = 0;
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int j = 0; j < V; ++j) mass += weight_units(log2_weight(v[a][j], m, c), shift);
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
+    }
+    if (lane == 0) {
+      out.mass[p] = mass;
+      out.max[p] = m;
+    }
+  }
+}
+
+// masses (and counts) of the classes of [begin, end), by the lanes of one wave, added into `mass` (and `count`)
+template <typename T>
+__device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, int end, float m, const Row& r, int shift,
+                                            uint64_t* mass, uint32_t* count) {
+  constexpr int V = Vec16<T>::n;
+  for_each_vec<T, 64>(x, begin, end, threadIdx.x & 63, [&](const float (&v)[V], int) {
+    uint64_t u[V];
+    double y[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      y[j] = log2_weight(v[j], m, r.c);
+      u[j] = weight_units(y[j], shift);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (u[j]) {
+        const int b = weight_bin(y[j]);
+        atomicAdd((unsigned long long*)&mass[b], (unsigned long long)u[j]);
+        if (r.k > 0) atomicAdd(&count[b], 1u);
+      }
+    }
+  });
+}
+
+// the row's classes: the sum of its segments' -> w.mass; every thread gets the whole mass
+template <typename T, int NT>
+__device__ __forceinline__ uint64_t sum_classes(const RowView<T>& v, RowWork<T, NT>& w) {
   __syncthreads();
-  return total;
+  uint64_t total = 0;
+  for (int b = threadIdx.x; b < kBins; b += NT) {
+    uint64_t s = 0;
+    for (int g = 0; g < v.n_seg; ++g) s += v.seg_hist[(size_t)g * kBins + b];
+    w.mass[b] = s;
+    total += s;
+  }
+  return group_sum<uint64_t, NT>(total, w.red64);
 }
 
 // Finds the class that reaches `need` (a count, or a mass) counted from class 0 -> w.bin and what lies above it.  The first
@@ -328,20 +447,23 @@ __device__ __forceinline__ void scan_classes(RowWork<T, NT>& w, bool by_mass, ui
       const uint64_t so = __shfl_up(si, off, 64);
       if (l >= off) { ci += co; si += so; }
     }
-    if (l == 0) w.bin = -1;
     uint32_t ca = ci - cs;   // above this lane's classes
     uint64_t sa = si - ss;
+    int bin = -1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const bool here = by_mass ? (sa < need && sa + s[j] >= need) : ((uint64_t)ca < need && (uint64_t)ca + c[j] >= need);
       if (here) {
-        w.bin = 4 * l + j;
+        bin = 4 * l + j;
         w.above_count = ca;
         w.above_mass = sa;
       }
       ca += c[j];
       sa += s[j];
     }
+    const uint64_t who = __ballot(bin >= 0);   // one lane, or none
+    bin = who ? __shfl(bin, __ffsll((unsigned long long)who) - 1, 64) : -1;
+    if (l == 0) w.bin = bin;
   }
   __syncthreads();
 }
@@ -352,23 +474,34 @@ struct Cut {
   uint64_t above;       // mass of the larger ones
 };
 
-// The value at which the count (or mass) counted from the top reaches `need`, inside class `bin` of the histogram.
+// The values of class `bin` -> w.list (as many as it takes; w.n is their number), their range -> w.lo, w.hi.
 template <typename T, int NT>
-__device__ __forceinline__ Cut refine(const T* __restrict__ x, int64_t A, float m, const Row& r, int shift,
-                                      RowWork<T, NT>& w, int bin, uint64_t above_mass, uint64_t above_count, bool by_mass,
-                                      uint64_t need) {
+__device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<T, NT>& w, int bin) {
+  constexpr int V = Vec16<T>::n;
   __syncthreads();
   if (threadIdx.x == 0) { w.n = 0; w.lo = 0xffffffffu; w.hi = 0; }
   __syncthreads();
+  // a little more than the class' range: two comparisons for almost all values, the class itself for the rest
+  const double step = 42.0 / kBins / v.r.c, slack = 1e-6 * (fabs((double)v.m) + (bin + 1) * step) + 1e-37;
+  const float top = (float)((double)v.m - bin * step + slack);
+  const float bottom = bin == kBins - 1 ? -INFINITY : (float)((double)v.m - (bin + 1) * step - slack);
   uint32_t lo = 0xffffffffu, hi = 0;
-  for_each<T, NT>(x, 0, A, threadIdx.x, [&](float v) {
-    const double y = log2_weight(v, m, r.c);
-    if (y >= kFloorLog2 && weight_bin(y) == bin) {
-      const uint32_t k = value_key(v);
-      lo = k < lo ? k : lo;
-      hi = k > hi ? k : hi;
-      const uint32_t at = atomicAdd(&w.n, 1u);
-      if (at < kList) w.list[at] = k;
+  for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int i) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (g[j] <= top && g[j] >= bottom) {
+        const double y = log2_weight(g[j], v.m, v.r.c);
+        if (y >= kFloorLog2 && weight_bin(y) == bin) {
+          const uint32_t k = value_key(g[j]);
+          lo = k < lo ? k : lo;
+          hi = k > hi ? k : hi;
+          const uint32_t at = atomicAdd(&w.n, 1u);
+          if (at < RowWork<T, NT>::kList) {
+            w.list[at] = k;
+            w.list_seg[at] = (uint8_t)(i / v.seg_len);
+          }
+        }
+      }
     }
   });
   if (hi != 0) {
@@ -376,223 +509,211 @@ __device__ __forceinline__ Cut refine(const T* __restrict__ x, int64_t A, float 
     atomicMax(&w.hi, hi);
   }
   __syncthreads();
-  lo = w.lo;
-  hi = w.hi;
+}
+
+// The value at which the count (or mass) counted from the top reaches `need`, inside the listed class.
+template <typename T, int NT>
+__device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<T, NT>& w, uint64_t above_mass, uint64_t above_count,
+                                      bool by_mass, uint64_t need) {
+  constexpr int V = Vec16<T>::n;
+  uint32_t lo = w.lo, hi = w.hi;
   const uint32_t n = w.n;
-  const bool listed = n <= kList;
   while (lo < hi) {   // at least 8 bits less each time
     int sh = 24 - __clz(hi - lo);
     if (sh < 0) sh = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += NT) { w.mass[i] = 0; w.count[i] = 0; }
     __syncthreads();
     auto add = [&](uint32_t k) {
       if (k >= lo && k <= hi) {
         const int b = (int)((hi - k) >> sh);
         atomicAdd(&w.count[b], 1u);
-        atomicAdd((unsigned long long*)&w.mass[b], (unsigned long long)weight_units(log2_weight(key_value(k), m, r.c), shift));
+        atomicAdd((unsigned long long*)&w.mass[b],
+                  (unsigned long long)weight_units(log2_weight(key_value(k), v.m, v.r.c), v.shift));
       }
     };
-    if (listed)
+    if (n <= RowWork<T, NT>::kList)
       for (uint32_t i = threadIdx.x; i < n; i += NT) add(w.list[i]);
     else
-      for_each<T, NT>(x, 0, A, threadIdx.x, [&](float v) { add(value_key(v)); });
+      for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) add(value_key(g[j]));
+      });
     scan_classes(w, by_mass, need - (by_mass ? above_mass : above_count));
     const int b = w.bin < 0 ? 0 : w.bin;   // it is there: the class as a whole reaches `need`
     above_mass += w.above_mass;
     above_count += w.above_count;
-    const uint32_t top = hi - ((uint32_t)b << sh);
-    const uint32_t width = (1u << sh) - 1;
+    const uint32_t top = hi - ((uint32_t)b << sh), width = (1u << sh) - 1;
     hi = top;
     lo = top - lo > width ? top - width : lo;
-    if (sh == 0) lo = hi;
-    __syncthreads();
   }
   Cut cut;
   cut.value = key_value(hi);
   cut.above = above_mass;
-  const uint64_t one = weight_units(log2_weight(cut.value, m, r.c), shift);
+  const uint64_t one = weight_units(log2_weight(cut.value, v.m, v.r.c), v.shift);
   cut.ties = by_mass ? (uint32_t)((need - above_mass + one - 1) / one) : (uint32_t)(need - above_count);
   return cut;
 }
 
-// the cut of top-k and top-p, from the row's histogram in w (which it uses up)
+// The cut of top-k and top-p, from the row's classes in w.mass, w.count.  `listed` is the class in w.list afterwards.
 template <typename T, int NT>
-__device__ __forceinline__ Cut find_cut(const T* __restrict__ x, int64_t A, float m, const Row& r, int shift, uint64_t total,
-                                        RowWork<T, NT>& w) {
-  Cut cut{-INFINITY, 0xffffffffu, 0};
+__device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<T, NT>& w, uint64_t total, int& listed) {
+  Cut cut{-INFINITY, 0, 0};
   uint64_t mass_k = total;
-  int bin_k = -1, bin_p = -1;
-  uint64_t am_k = 0, am_p = 0, ac_k = 0, ac_p = 0;
-  if (r.k > 1) {
-    scan_classes(w, false, (uint64_t)r.k);
-    bin_k = w.bin;
-    am_k = w.above_mass;
-    ac_k = w.above_count;
-  }
-  uint64_t need = 0;
-  if (bin_k >= 0) {   // the histogram is needed again for top-p: scan for it before it is used up
-    if (r.top_p < 1.f) {
-      // mass_k lies between the masses above and through class bin_k; the class of the top-p border is known
-      // only when mass_k is.  Keep the classes in registers of the first wave's lanes.
-      uint64_t keep_m[4];
-      uint32_t keep_c[4];
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = 4 * (threadIdx.x & 63) + j;
-        keep_m[j] = w.mass[i];
-        keep_c[j] = w.count[i];
-      }
-      cut = refine(x, A, m, r, shift, w, bin_k, am_k, ac_k, false, (uint64_t)r.k);
-      mass_k = cut.above + (uint64_t)cut.ties * weight_units(log2_weight(cut.value, m, r.c), shift);
-      __syncthreads();
-      if (threadIdx.x < 64) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w.mass[4 * threadIdx.x + j] = keep_m[j];
-          w.count[4 * threadIdx.x + j] = keep_c[j];
-        }
-      }
-    } else {
-      return refine(x, A, m, r, shift, w, bin_k, am_k, ac_k, false, (uint64_t)r.k);
+  listed = -1;
+  if (v.r.k > 0) {
+    scan_classes(w, false, (uint64_t)v.r.k);
+    const int bin = w.bin;
+    if (bin >= 0) {   // else fewer than k have any weight
+      const uint64_t am = w.above_mass, ac = w.above_count;
+      gather_class(v, w, bin);
+      listed = bin;
+      cut = refine(v, w, am, ac, false, (uint64_t)v.r.k);
+      mass_k = cut.above + (uint64_t)cut.ties * weight_units(log2_weight(cut.value, v.m, v.r.c), v.shift);
     }
   }
-  if (r.top_p < 1.f) {
-    need = top_p_mass(r.top_p, mass_k);
+  if (v.r.top_p < 1.f) {
+    if (listed >= 0) sum_classes(v, w);   // they were used up
+    const uint64_t need = top_p_mass(v.r.top_p, mass_k);
     scan_classes(w, true, need);
-    bin_p = w.bin;
-    am_p = w.above_mass;
-    ac_p = w.above_count;
-    const Cut p = refine(x, A, m, r, shift, w, bin_p < 0 ? 0 : bin_p, am_p, ac_p, true, need);
+    const int bin = w.bin < 0 ? 0 : w.bin;   // it is there: need <= total
+    const uint64_t am = w.above_mass;
+    if (bin != listed) gather_class(v, w, bin);
+    listed = bin;
+    const Cut p = refine(v, w, am, 0, true, need);
     if (p.value > cut.value || (p.value == cut.value && p.ties < cut.ties)) cut = p;
   }
   return cut;
 }
 
-// What is kept of [begin, end), by the lanes of one wave: mass of the values above the cut, number of values at the cut,
-// and (all) the mass of everything.
-template <typename T>
-__device__ __forceinline__ void kept_mass(const T* __restrict__ x, int64_t begin, int64_t end, float m, const Row& r,
-                                          int shift, const Cut& cut, bool want_all, uint64_t& mass, uint32_t& ties,
-                                          uint64_t& all) {
-  uint64_t s = 0, a = 0;
-  uint32_t t = 0;
-  for_each<T, 64>(x, begin, end, threadIdx.x & 63, [&](float v) {
-    const bool above = v > cut.value;
-    t += v == cut.value;
-    if (above || want_all) {
-      const double y = log2_weight(v, m, r.c);
-      if (y >= kFloorLog2) {
-        const uint64_t u = weight_units(y, shift);
-        a += u;
-        if (above && y >= r.ymin) s += u;
-      }
-    }
-  });
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    s += __shfl_xor(s, off, 64);
-    a += __shfl_xor(a, off, 64);
-    t += __shfl_xor(t, off, 64);
-  }
-  mass = s;
-  ties = t;
-  all = a;
-}
-
-// the segments of a row that are summed one by one: `n` of `len` elements
-__device__ __forceinline__ int64_t segment_length(int64_t A, int n) {
-  const int64_t len = (A + n - 1) / n;
-  return (len + 511) / 512 * 512;
-}
-
-// The draw: seg_mass / seg_ties hold n segments' sums.  Thread-uniform result: the segment, and the target and the ties left
-// at its beginning.  Then the segment is scanned in index order.
+// The kept mass and the values at the cut of every segment -> w.seg_mass, w.seg_ties.
 template <typename T, int NT>
-__device__ __forceinline__ void pick(const T* __restrict__ x, int64_t A, float m, const Row& r, const SampleArgs& q,
-                                     int64_t row, const Cut& cut, uint64_t total, const uint64_t* seg_mass,
-                                     const uint32_t* seg_ties, int n, int64_t len, RowWork<T, NT>& w) {
-  constexpr int V = Vec16<T>::n;
-  const double y_cut = log2_weight(cut.value, m, r.c);
-  // the values at the cut are kept if min_p keeps them
-  const uint64_t one = cut.value > -INFINITY && y_cut >= r.ymin ? weight_units(y_cut, q.shift) : 0;
-  uint64_t mass = 0;
-  uint32_t left = one ? cut.ties : 0;
-  for (int s = 0; s < n; ++s) {
-    const uint32_t t = seg_ties[s] < left ? seg_ties[s] : left;
-    mass += seg_mass[s] + (uint64_t)t * one;
-    left -= t;
-  }
-  uint64_t target = draw_target(q.uniforms[row], mass);
-  left = one ? cut.ties : 0;
-  int s = 0;
-  for (; s < n - 1; ++s) {
-    const uint32_t t = seg_ties[s] < left ? seg_ties[s] : left;
-    const uint64_t here = seg_mass[s] + (uint64_t)t * one;
-    if (here > target) break;
-    target -= here;
-    left -= t;
-  }
-  const int64_t begin = s * len, end = begin + len < A ? begin + len : A;
+__device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<T, NT>& w, const Cut& cut, int listed) {
+  constexpr int V = Vec16<T>::n, kWaves = NT / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int64_t base = begin; base < end; base += (int64_t)NT * V) {
-    const int64_t i0 = base + (int64_t)threadIdx.x * V;
-    float v[V];
-    uint64_t u[V];
-    uint32_t tie = 0;
-    bool full = i0 + V <= end;
-    if (full) {
-      Vec16<T> raw;
-      raw.load(x + i0);
-      raw.unpack(v);
-    } else {
+  const double y_cut = cut.value > -INFINITY ? log2_weight(cut.value, v.m, v.r.c) : kFloorLog2;
+  const int bin = weight_bin(fmax(y_cut, v.r.ymin));   // above it everything is kept, below it nothing
+  if (bin != listed) gather_class(v, w, bin);
+  __syncthreads();
+  const uint32_t n = w.n;
+  if (n <= RowWork<T, NT>::kList) {
+    for (int s = wave; s < v.n_seg; s += kWaves) {
+      uint64_t mass = 0;
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[j] = i0 + j < end ? to_f32(x[i0 + j]) : -INFINITY;
-    }
+      for (int j = 0; j < 4; ++j)
+        if (64 * j + lane < bin) mass += v.seg_hist[(size_t)s * kBins + 64 * j + lane];
 #pragma unroll
-    for (int j = 0; j < V; ++j) tie += one && v[j] == cut.value;
-    uint32_t ti = tie;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = __shfl_up(ti, off, 64);
-      if (lane >= off) ti += o;
-    }
-    uint32_t tie_before = ti - tie, tie_all = 0;
-    if constexpr (NT > 64) {
-      __syncthreads();
-      if (lane == 63) w.red32[wave] = ti;
-      __syncthreads();
-#pragma unroll
-      for (int o = 0; o < NT / 64; ++o) {
-        if (o < wave) tie_before += w.red32[o];
-        tie_all += w.red32[o];
+      for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
+      if (lane == 0) {
+        w.seg_mass[s] = mass;
+        w.seg_ties[s] = 0;
       }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += NT) {
+      const float x = key_value(w.list[i]);
+      const int s = w.list_seg[i];
+      const double y = log2_weight(x, v.m, v.r.c);
+      if (x == cut.value)
+        atomicAdd(&w.seg_ties[s], 1u);
+      else if (x > cut.value && y >= v.r.ymin)
+        atomicAdd((unsigned long long*)&w.seg_mass[s], (unsigned long long)weight_units(y, v.shift));
+    }
+  } else {   // a flat row: over the whole of it again
+    for (int s = wave; s < v.n_seg; s += kWaves) {
+      const int begin = s * v.seg_len < v.A ? s * v.seg_len : v.A, end = begin + v.seg_len < v.A ? begin + v.seg_len : v.A;
+      uint64_t mass = 0;
+      uint32_t ties = 0;
+      for_each_vec<T, 64>(v.x, begin, end, lane, [&](const float (&g)[V], int) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const double y = log2_weight(g[j], v.m, v.r.c);
+          const uint64_t u = weight_units(y, v.shift);
+          mass += g[j] > cut.value && y >= v.r.ymin ? u : 0;
+          ties += g[j] == cut.value;
+        }
+      });
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) {
+        mass += __shfl_xor(mass, off, 64);
+        ties += __shfl_xor(ties, off, 64);
+      }
+      if (lane == 0) {
+        w.seg_mass[s] = mass;
+        w.seg_ties[s] = ties;
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// Scans [begin, end) in index order for the first action whose running kept mass exceeds target; of the values at the cut
+// the first `left` are kept, each with `one` (0: none are).  True if it was there, else `seen` is the mass that was.
+template <typename T, int NT>
+__device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row, int begin,
+                                          int end, const Cut& cut, uint64_t one, uint32_t left, uint64_t target,
+                                          uint64_t total, uint64_t& seen) {
+  constexpr int V = Vec16<T>::n;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  seen = 0;
+  for (int base = begin; base < end; base += NT * V) {
+    const int i0 = base + (int)threadIdx.x * V;
+    float g[V];
+    uint64_t u[V];
+    if (i0 + V <= end) {
+      Vec16<T> raw;
+      raw.load(v.x + i0);
+      raw.unpack(g);
     } else {
-      tie_all = __shfl(ti, 63, 64);
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = i0 + j < end ? to_f32(v.x[i0 + j]) : -INFINITY;
+    }
+    uint32_t tie_before = 0, tie_all = 0;
+    if (one) {   // the same for the whole group
+      uint32_t tie = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) tie += g[j] == cut.value;
+      uint32_t run = tie;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const uint32_t o = __shfl_up(run, off, 64);
+        if (lane >= off) run += o;
+      }
+      tie_before = run - tie;
+      if constexpr (NT > 64) {
+        __syncthreads();
+        if (lane == 63) w.red32[wave] = run;
+        __syncthreads();
+#pragma unroll
+        for (int o = 0; o < NT / 64; ++o) {
+          if (o < wave) tie_before += w.red32[o];
+          tie_all += w.red32[o];
+        }
+      } else {
+        tie_all = __shfl(run, 63, 64);
+      }
     }
     uint64_t sum = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      u[j] = 0;
-      if (v[j] > cut.value) {
-        const double y = log2_weight(v[j], m, r.c);
-        if (y >= r.ymin) u[j] = weight_units(y, q.shift);
-      } else if (one && v[j] == cut.value) {
+      const double y = log2_weight(g[j], v.m, v.r.c);
+      u[j] = g[j] > cut.value && y >= v.r.ymin ? weight_units(y, v.shift) : 0;
+      if (one && g[j] == cut.value) {
         if (tie_before < left) u[j] = one;
         ++tie_before;
       }
       sum += u[j];
     }
-    uint64_t si = sum;
+    uint64_t run = sum;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const uint64_t o = __shfl_up(si, off, 64);
-      if (lane >= off) si += o;
+      const uint64_t o = __shfl_up(run, off, 64);
+      if (lane >= off) run += o;
     }
-    uint64_t before = si - sum, here = 0;
+    uint64_t before = run - sum, here = 0;
     if constexpr (NT > 64) {
       __syncthreads();
-      if (lane == 63) w.red64[wave] = si;
+      if (lane == 63) w.red64[wave] = run;
       __syncthreads();
 #pragma unroll
       for (int o = 0; o < NT / 64; ++o) {
@@ -600,7 +721,7 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int64_t A, float m
         here += w.red64[o];
       }
     } else {
-      here = __shfl(si, 63, 64);
+      here = __shfl(run, 63, 64);
     }
     if (here > target) {   // it is in this tile, and one thread has it
       if (before <= target && before + sum > target) {
@@ -608,15 +729,116 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int64_t A, float m
         for (int j = 0; j < V; ++j) {
           if (before <= target && before + u[j] > target) {
             q.actions[row] = i0 + j;
-            q.log_probs[row] = log_prob_of(v[j], m, r, total, q.shift);
+            q.log_probs[row] = log_prob_of(g[j], v.m, v.r, total, v.shift);
           }
           before += u[j];
         }
       }
-      return;
+      return true;
     }
     target -= here;
+    seen += here;
     left -= tie_all < left ? tie_all : left;
+  }
+  return false;
+}
+
+// The draw of a filtered row, from its segments' classes (v.seg_hist) and, for top-k, the row's counts in w.count.
+template <typename T, int NT>
+__device__ __forceinline__ void draw_filtered(const RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row) {
+  const uint64_t total = sum_classes(v, w);
+  int listed;
+  const Cut cut = find_cut(v, w, total, listed);
+  sum_segments(v, w, cut, listed);
+  const double y_cut = cut.value > -INFINITY ? log2_weight(cut.value, v.m, v.r.c) : 0.0;
+  // the values at the cut are kept if min_p keeps them
+  const uint64_t one = cut.value > -INFINITY && y_cut >= v.r.ymin ? weight_units(y_cut, v.shift) : 0;
+  uint64_t mass = 0;
+  uint32_t left = one ? cut.ties : 0;
+  for (int s = 0; s < v.n_seg; ++s) {
+    const uint32_t t = w.seg_ties[s] < left ? w.seg_ties[s] : left;
+    mass += w.seg_mass[s] + (uint64_t)t * one;
+    left -= t;
+  }
+  uint64_t target = draw_target(q.uniforms[row], mass);
+  left = one ? cut.ties : 0;
+  int s = 0;
+  for (; s < v.n_seg - 1; ++s) {
+    const uint32_t t = w.seg_ties[s] < left ? w.seg_ties[s] : left;
+    const uint64_t here = w.seg_mass[s] + (uint64_t)t * one;
+    if (here > target) break;
+    target -= here;
+    left -= t;
+  }
+  const int begin = s * v.seg_len, end = begin + v.seg_len < v.A ? begin + v.seg_len : v.A;
+  uint64_t seen;
+  scan_draw(v, w, q, row, begin, end, cut, one, left, target, total, seen);
+}
+
+// The draw of a row without filters, from the sums of its pieces (n <= NT of them; v.m is not known yet).
+template <typename T, int NT>
+__device__ __forceinline__ void draw_pieces(RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row, const Pieces& p,
+                                            int n) {
+  constexpr int kLen = piece_length<T>();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x;
+  const uint64_t raw = i < n ? p.mass[i] : 0;
+  const float ref = i < n ? p.max[i] : -INFINITY;
+  bool bad = false;
+  v.m = group_max<NT>(ref, bad, w.red32);
+  // the piece's mass relative to the row's maximum: exact where that is the piece's own, rounded to 53 bits elsewhere
+  const double y = ref > -INFINITY ? log2_weight(ref, v.m, v.r.c) : -1e9;
+  const uint64_t mass = y == 0.0 ? raw : y >= kFloorLog2 ? (uint64_t)rint((double)raw * exp2(y)) : 0;
+  uint64_t run = mass;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint64_t o = __shfl_up(run, off, 64);
+    if (lane >= off) run += o;
+  }
+  uint64_t before = run - mass, total = 0;
+  if constexpr (NT > 64) {
+    __syncthreads();
+    if (lane == 63) w.red64[wave] = run;
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < NT / 64; ++o) {
+      if (o < wave) before += w.red64[o];
+      total += w.red64[o];
+    }
+  } else {
+    total = __shfl(run, 63, 64);
+  }
+  const uint64_t target = draw_target(q.uniforms[row], total);
+  if (before <= target && before + mass > target) {   // one thread
+    w.found = i;
+    w.found_target = target - before;
+  }
+  __syncthreads();
+  const int begin = w.found * kLen, end = begin + kLen < v.A ? begin + kLen : v.A;
+  const Cut all{-INFINITY, 0, 0};
+  uint64_t seen;
+  // The weights of the piece, each rounded relative to the row's maximum, may sum to a few units less than its mass did;
+  // its largest is at least one unit.
+  if (!scan_draw(v, w, q, row, begin, end, all, 0, 0, w.found_target, total, seen))
+    scan_draw(v, w, q, row, begin, end, all, 0, 0, seen - 1, total, seen);
+}
+
+// the largest logit, the first among equals
+template <typename T, int NT>
+__device__ __forceinline__ void draw_greedy(const RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row) {
+  constexpr int V = Vec16<T>::n;
+  if (threadIdx.x == 0) w.found = 0x7fffffff;
+  __syncthreads();
+  int first = 0x7fffffff;
+  for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int i) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (g[j] == v.m && i + j < first) first = i + j;
+  });
+  if (first != 0x7fffffff) atomicMin(&w.found, first);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    q.actions[row] = w.found;
+    q.log_probs[row] = 0.f;
   }
 }
 
@@ -631,39 +853,47 @@ __device__ __forceinline__ bool no_draw(const SampleArgs& q, int64_t row, float 
   return true;
 }
 
-// A workgroup per row: the maximum, the cut where a filter asks for one, the kept mass of each wave's segment, the draw.
+// `n` segments of a row: a multiple of every vector and of the loads in flight
+__host__ __device__ __forceinline__ int segment_length(int A, int n) { return ((A + n - 1) / n + 511) / 512 * 512; }
+
+// A workgroup per row.
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void sample_row_kernel(const T* __restrict__ logits, int64_t stride, int64_t A, SampleArgs q) {
+__global__ __launch_bounds__(NT) void sample_row_kernel(const T* __restrict__ logits, int64_t stride, int A, SampleArgs q) {
   __shared__ RowWork<T, NT> w;
   constexpr int kWaves = NT / 64;
   const int64_t row = blockIdx.x;
-  const T* x = logits + row * stride;
-  const Row r = row_settings(q, row);
-  bool bad;
-  const float m = part_max<T, NT>(x, 0, A, bad, w.red32);
-  if (no_draw(q, row, m, bad)) return;
-  Cut cut{-INFINITY, 0, 0};
-  uint64_t total = 0;
-  const bool hist = needs_histogram(r);
-  if (hist) {
-    total = group_sum<uint64_t, NT>(part_histogram(x, 0, A, m, r, q.shift, w), w.red64);
-    cut = find_cut(x, A, m, r, q.shift, total, w);
-  } else if (r.k == 1) {
-    cut = Cut{m, 1, 0};
-  }
-  const int64_t len = segment_length(A, kWaves);
   const int wave = threadIdx.x >> 6;
-  const int64_t begin = wave * len < A ? wave * len : A, end = begin + len < A ? begin + len : A;
-  uint64_t mass, all;
-  uint32_t ties;
-  kept_mass(x, begin, end, m, r, q.shift, cut, !hist && !r.greedy, mass, ties, all);
-  if ((threadIdx.x & 63) == 0) {
-    w.seg_mass[wave] = mass;
-    w.seg_ties[wave] = ties;
+  RowView<T> v;
+  v.x = logits + row * stride;
+  v.A = A;
+  v.r = row_settings(q, row);
+  v.shift = q.shift;
+  bool bad;
+  if (!v.r.greedy && !filtered(v.r)) {
+    const int n = (A + piece_length<T>() - 1) / piece_length<T>();
+    const Pieces p{w.piece.mass, w.piece.max};
+    sum_pieces(v.x, A, v.r.c, v.shift, 0, n, wave, kWaves, p, bad);
+    // the largest piece's maximum decides whether there is anything to draw; the barriers order the pieces' sums too
+    __syncthreads();
+    float m = (int)threadIdx.x < n ? p.max[threadIdx.x] : -INFINITY;
+    m = group_max<NT>(m, bad, w.red32);
+    if (no_draw(q, row, m, bad)) return;
+    draw_pieces(v, w, q, row, p, n);
+    return;
   }
-  if (!hist) total = group_sum<uint64_t, NT>((threadIdx.x & 63) == 0 ? all : 0, w.red64);
+  v.m = part_max<T, NT>(v.x, 0, A, bad);
+  v.m = group_max<NT>(v.m, bad, w.red32);
+  if (no_draw(q, row, v.m, bad)) return;
+  if (v.r.greedy) return draw_greedy(v, w, q, row);
+  v.n_seg = kWaves;
+  v.seg_len = segment_length(A, kWaves);
+  v.seg_hist = &w.wave_mass[0][0];
+  for (int i = threadIdx.x; i < kWaves * kBins; i += NT) (&w.wave_mass[0][0])[i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += NT) w.count[i] = 0;
   __syncthreads();
-  pick(x, A, m, r, q, row, cut, total, w.seg_mass, w.seg_ties, kWaves, len, w);
+  const int begin = wave * v.seg_len < A ? wave * v.seg_len : A, end = begin + v.seg_len < A ? begin + v.seg_len : A;
+  add_classes(v.x, begin, end, v.m, v.r, v.shift, w.wave_mass[wave], w.count);
+  draw_filtered(v, w, q, row);
 }
 
 static inline int sample_shift(int64_t A) {
@@ -682,11 +912,11 @@ static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, con
     else if (lanes == 32) sample_small_kernel<T, 32><<<grid, 256, 0, s>>>(logits, stride, B, (int)A, q);
     else sample_small_kernel<T, 64><<<grid, 256, 0, s>>>(logits, stride, B, (int)A, q);
   } else if (A <= 2048) {
-    sample_row_kernel<T, 64><<<(int)B, 64, 0, s>>>(logits, stride, A, q);
+    sample_row_kernel<T, 64><<<(int)B, 64, 0, s>>>(logits, stride, (int)A, q);
   } else if (A <= 16384) {
-    sample_row_kernel<T, 256><<<(int)B, 256, 0, s>>>(logits, stride, A, q);
+    sample_row_kernel<T, 256><<<(int)B, 256, 0, s>>>(logits, stride, (int)A, q);
   } else {
-    sample_row_kernel<T, 1024><<<(int)B, 1024, 0, s>>>(logits, stride, A, q);
+    sample_row_kernel<T, 1024><<<(int)B, 1024, 0, s>>>(logits, stride, (int)A, q);
   }
   return check_launch();
 }
