@@ -21,8 +21,8 @@
 //               values in LDS, by the same histogram over ever fewer bits (or on the row itself, where a flat row puts
 //               more values into one class than the list takes).  The classes above the border and the list give the
 //               kept mass of every segment, and the segment that the draw falls into is scanned.
-//   few rows    are cut into parts, one workgroup each, for the passes over the whole row; a workgroup per row joins
-//               what they leave in the workspace and goes on as above.
+// Rows of up to 2,048 actions do that in one wave each.  Above, every pass over the rows is a launch of its own over segments of
+// all rows, which fills the card whether the rows are many or few and long, and a workgroup per row finishes.
 #include "common.hpp"
 #include "logits_common.hpp"
 
@@ -204,23 +204,24 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
 // Longer rows: a workgroup of NT threads for a row or a part of one.
 
 // f(v, i) for the vectors of [begin, end) of a row, by the threads tid < NT, four loads in flight: v are the V elements from
-// i on; what lies behind the end is -inf, which has no weight.  begin is a multiple of V.
+// i on; what lies behind the end is -inf, which has no weight.  begin is a multiple of V.  All threads make all rounds.
 template <typename T, int NT, typename F>
 __device__ __forceinline__ void for_each_vec(const T* __restrict__ x, int begin, int end, int tid, F&& f) {
   constexpr int V = Vec16<T>::n;
-  int i = begin + tid * V;
-  for (; i + 3 * NT * V + V <= end; i += 4 * NT * V) {
+  int base = begin;
+  for (; base + 4 * NT * V <= end; base += 4 * NT * V) {
     Vec16<T> v[4];
 #pragma unroll
-    for (int a = 0; a < 4; ++a) v[a].load(x + i + a * NT * V);
+    for (int a = 0; a < 4; ++a) v[a].load(x + base + (a * NT + tid) * V);
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       float g[V];
       v[a].unpack(g);
-      f(g, i + a * NT * V);
+      f(g, base + (a * NT + tid) * V);
     }
   }
-  for (; i < end; i += NT * V) {
+  for (; base < end; base += NT * V) {
+    const int i = base + tid * V;
     float g[V];
     if (i + V <= end) {
       Vec16<T> v;
@@ -238,32 +239,26 @@ __device__ __forceinline__ void for_each_vec(const T* __restrict__ x, int begin,
 template <typename T>
 __host__ __device__ constexpr int piece_length() { return 64 * 4 * 16 / (int)sizeof(T); }
 
-struct Pieces {          // of one row, in LDS or in the workspace
+struct Pieces {          // of one row
   uint64_t* mass;
-  float* max;
+  float* max;            // NaN: a NaN or +inf was among them
 };
 
-template <typename T, int NT>
+template <int NT>
 struct RowWork {
   static constexpr int kWaves = NT / 64;
-  static constexpr int kList = NT == 1024 ? 4096 : NT == 256 ? 2048 : 1024;
-  static constexpr int kPieces = NT == 1024 ? 1024 : NT == 256 ? 16 : 2;
-  union {
-    uint64_t wave_mass[kWaves][kBins];   // the histogram of each wave's segment
-    struct {
-      uint64_t mass[kPieces];
-      float max[kPieces];
-    } piece;
-  };
+  static constexpr int kList = NT == 64 ? 1024 : 512;   // of each wave
   uint64_t mass[kBins];                  // of the row, or of the class that is being taken apart
   uint32_t count[kBins];
-  uint32_t list[kList];                  // the values (keys) of a class and the segments that they are in
-  uint8_t list_seg[kList];
+  uint32_t list[kWaves][kList];          // the values (keys; 0: none) of a class and the segments that they are in
+  uint8_t list_seg[kWaves][kList];
+  uint32_t list_n[kWaves];
   uint64_t seg_mass[kMaxParts];
   uint32_t seg_ties[kMaxParts];
   uint64_t red64[kWaves];
   uint32_t red32[kWaves];
-  uint32_t lo, hi, n;                    // of the listed class
+  uint32_t lo, hi;                       // of the listed class
+  bool listed;                           // whether the lists took all of it
   int bin;                               // what the scan found
   uint64_t above_mass;
   uint32_t above_count;
@@ -280,7 +275,8 @@ struct RowView {
   Row r;
   int shift;
   int n_seg, seg_len;                    // segment s: [s * seg_len, ...); seg_len is a multiple of every vector
-  const uint64_t* seg_hist;              // [n_seg][kBins]
+  const uint64_t* seg_hist;              // [n_seg][kBins]: masses of the classes
+  const uint32_t* seg_count;             // and counts
 };
 
 template <typename X, int NT>
@@ -298,97 +294,95 @@ __device__ __forceinline__ X group_sum(X v, X* lds) {   // every thread gets the
   return v;
 }
 
-// the largest value over the group, and whether any thread saw a NaN or +inf
+// the largest value over the group; NaN if any thread's is
 template <int NT>
-__device__ __forceinline__ float group_max(float m, bool& bad, uint32_t* lds) {
-  m = wave_max_f32(m);
-  bad = __any(bad);
+__device__ __forceinline__ float group_max(float m, uint32_t* lds) {
+  const bool bad = __any(m != m);
+  m = bad ? __builtin_nanf("") : wave_max_f32(m);
   if constexpr (NT > 64) {
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = bad ? 0xffffffffu : value_key(m);   // no value has that key
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = bad ? 0xffffffffu : value_key(m);   // no number has that key
     __syncthreads();
     uint32_t k = lds[0];
 #pragma unroll
     for (int o = 1; o < NT / 64; ++o) k = lds[o] > k ? lds[o] : k;
-    bad = k == 0xffffffffu;
-    m = key_value(k);
+    m = k == 0xffffffffu ? __builtin_nanf("") : key_value(k);
   }
   return m;
 }
 
-// this thread's share of the maximum of [begin, end)
-template <typename T, int NT>
-__device__ __forceinline__ float part_max(const T* __restrict__ x, int begin, int end, bool& bad) {
-  float m = -INFINITY;
-  bool b = false;
-  for_each_vec<T, NT>(x, begin, end, threadIdx.x, [&](const float (&v)[Vec16<T>::n], int) {
-#pragma unroll
-    for (int j = 0; j < Vec16<T>::n; ++j) {
-      b |= !(v[j] < INFINITY);
-      m = fmaxf(m, v[j]);
-    }
-  });
-  bad = b;
-  return m;
-}
-
-// The pieces [first, last) of a row, one after the other by each of the waves `wave` of `waves`: their maxima and their
-// masses relative to these.  bad: a NaN or +inf was seen.  -inf as a maximum: a piece without a legal action.
+// The pieces [first, last) of a row, one after the other by each of the waves `wave` of `waves`: their maxima and, with
+// SUM, their masses relative to these.
 template <typename T>
 __device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, double c, int shift, int first, int last, int wave,
-                                           int waves, const Pieces& out, bool& bad) {
+                                           int waves, const Pieces& out, bool sum) {
   constexpr int V = Vec16<T>::n, kLen = piece_length<T>();
   const int lane = threadIdx.x & 63;
-  bad = false;
   for (int p = first + wave; p < last; p += waves) {
     const int base = p * kLen + lane * V;
-    float v[4][V];
+    Vec16<T> raw[4];
     if (p * kLen + kLen <= A) {
-      Vec16<T> raw[4];
 #pragma unroll
       for (int a = 0; a < 4; ++a) raw[a].load(x + base + a * 64 * V);
-#pragma unroll
-      for (int a = 0; a < 4; ++a) raw[a].unpack(v[a]);
     } else {
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+      for (int a = 0; a < 4; ++a) {
+        float g[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           const int i = base + a * 64 * V + j;
-          v[a][j] = i < A ? to_f32(x[i]) : -INFINITY;
+          g[j] = i < A ? to_f32(x[i]) : -INFINITY;
         }
+        raw[a].pack(g);   // exact: they came from this type
+      }
     }
     float m = -INFINITY;
+    bool bad = false;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        bad |= !(v[a][j] < INFINITY);
-        m = fmaxf(m, v[a][j]);
+        const float g = raw[a].get(j);
+        bad |= !(g < INFINITY);
+        m = fmaxf(m, g);
       }
-    m = wave_max_f32(m);
-    uint64_t mass = 0;
-    if (m > -INFINITY) {
+    m = group_max<64>(bad ? __builtin_nanf("") : m, nullptr);
+    if (sum) {
+      uint64_t mass = 0;
+      if (m > -INFINITY) {
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < 4; ++a)
 #pragma unroll
-        for (int j = 0; j < V; ++j) mass += weight_units(log2_weight(v[a][j], m, c), shift);
+          for (int j = 0; j < V; ++j) mass += weight_units(log2_weight(raw[a].get(j), m, c), shift);
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
+        for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
+      }
+      if (lane == 0) out.mass[p] = mass;
     }
-    if (lane == 0) {
-      out.mass[p] = mass;
-      out.max[p] = m;
-    }
+    if (lane == 0) out.max[p] = m;
   }
 }
 
-// masses (and counts) of the classes of [begin, end), by the lanes of one wave, added into `mass` (and `count`)
-template <typename T>
+// the row's maximum, from those of its pieces
+template <typename T, int NT>
+__device__ __forceinline__ float row_max(const Pieces& p, int A, uint32_t* lds) {
+  const int n = (A + piece_length<T>() - 1) / piece_length<T>();
+  float m = -INFINITY;
+  bool bad = false;
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const float o = p.max[i];
+    bad |= o != o;
+    m = fmaxf(m, o);
+  }
+  return group_max<NT>(bad ? __builtin_nanf("") : m, lds);
+}
+
+// masses (and counts, for top-k) of the classes of [begin, end), added into `mass` and `count` by NT threads
+template <typename T, int NT>
 __device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, int end, float m, const Row& r, int shift,
                                             uint64_t* mass, uint32_t* count) {
   constexpr int V = Vec16<T>::n;
-  for_each_vec<T, 64>(x, begin, end, threadIdx.x & 63, [&](const float (&v)[V], int) {
+  for_each_vec<T, NT>(x, begin, end, threadIdx.x, [&](const float (&v)[V], int) {
     uint64_t u[V];
     double y[V];
 #pragma unroll
@@ -407,15 +401,45 @@ __device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, 
   });
 }
 
-// the row's classes: the sum of its segments' -> w.mass; every thread gets the whole mass
+// the row's classes: the sum of its segments' -> w.mass, w.count; every thread gets the whole mass
 template <typename T, int NT>
-__device__ __forceinline__ uint64_t sum_classes(const RowView<T>& v, RowWork<T, NT>& w) {
+__device__ __forceinline__ uint64_t sum_classes(const RowView<T>& v, RowWork<NT>& w) {
+  constexpr int kGroups = NT > kBins ? NT / kBins : 1;   // of segments, side by side
   __syncthreads();
+  if constexpr (kGroups > 1) {
+    if (threadIdx.x < kBins) { w.mass[threadIdx.x] = 0; w.count[threadIdx.x] = 0; }
+    __syncthreads();
+  }
   uint64_t total = 0;
-  for (int b = threadIdx.x; b < kBins; b += NT) {
+  for (int b = threadIdx.x % kBins; b < kBins; b += NT) {
     uint64_t s = 0;
-    for (int g = 0; g < v.n_seg; ++g) s += v.seg_hist[(size_t)g * kBins + b];
-    w.mass[b] = s;
+    uint32_t c = 0;
+    int g = threadIdx.x / kBins;
+    for (; g + 7 * kGroups < v.n_seg; g += 8 * kGroups) {   // eight loads in flight
+      uint64_t t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = v.seg_hist[(g + j * kGroups) * kBins + b];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += t[j];
+      if (v.r.k > 0) {
+        uint32_t n[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n[j] = v.seg_count[(g + j * kGroups) * kBins + b];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) c += n[j];
+      }
+    }
+    for (; g < v.n_seg; g += kGroups) {
+      s += v.seg_hist[g * kBins + b];
+      if (v.r.k > 0) c += v.seg_count[g * kBins + b];
+    }
+    if constexpr (kGroups > 1) {
+      atomicAdd((unsigned long long*)&w.mass[b], (unsigned long long)s);
+      atomicAdd(&w.count[b], c);
+    } else {
+      w.mass[b] = s;
+      w.count[b] = c;
+    }
     total += s;
   }
   return group_sum<uint64_t, NT>(total, w.red64);
@@ -423,8 +447,8 @@ __device__ __forceinline__ uint64_t sum_classes(const RowView<T>& v, RowWork<T, 
 
 // Finds the class that reaches `need` (a count, or a mass) counted from class 0 -> w.bin and what lies above it.  The first
 // wave scans, four classes a lane.  bin = -1: the classes together do not reach it.
-template <typename T, int NT>
-__device__ __forceinline__ void scan_classes(RowWork<T, NT>& w, bool by_mass, uint64_t need) {
+template <int NT>
+__device__ __forceinline__ void scan_classes(RowWork<NT>& w, bool by_mass, uint64_t need) {
   __syncthreads();
   if (threadIdx.x < 64) {
     const int l = threadIdx.x;
@@ -474,36 +498,71 @@ struct Cut {
   uint64_t above;       // mass of the larger ones
 };
 
-// The values of class `bin` -> w.list (as many as it takes; w.n is their number), their range -> w.lo, w.hi.
+// f(key, segment) for the listed class, if the lists took it
+template <int NT, typename F>
+__device__ __forceinline__ void for_listed(RowWork<NT>& w, F&& f) {
+  const int wave = threadIdx.x >> 6;
+  const uint32_t n = w.list_n[wave];
+  for (uint32_t i = threadIdx.x & 63; i < n; i += 64) f(w.list[wave][i], (int)w.list_seg[wave][i]);
+}
+
+// The values of class `bin` -> w.list (w.listed: all of them), their range -> w.lo, w.hi.
 template <typename T, int NT>
-__device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<T, NT>& w, int bin) {
-  constexpr int V = Vec16<T>::n;
+__device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<NT>& w, int bin) {
+  constexpr int V = Vec16<T>::n, kList = RowWork<NT>::kList;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
-  if (threadIdx.x == 0) { w.n = 0; w.lo = 0xffffffffu; w.hi = 0; }
-  __syncthreads();
-  // a little more than the class' range: two comparisons for almost all values, the class itself for the rest
+  if (threadIdx.x == 0) { w.listed = true; w.lo = 0xffffffffu; w.hi = 0; }
+  // A little more than the class' range: one comparison for a load's values together where they are all below it, else two
+  // for each.  A wave appends what it finds to a list of its own; whether it is of the class is seen afterwards, on
+  // the list (float64 in this loop would run for every second load of a wave).
   const double step = 42.0 / kBins / v.r.c, slack = 1e-6 * (fabs((double)v.m) + (bin + 1) * step) + 1e-37;
   const float top = (float)((double)v.m - bin * step + slack);
-  const float bottom = bin == kBins - 1 ? -INFINITY : (float)((double)v.m - (bin + 1) * step - slack);
-  uint32_t lo = 0xffffffffu, hi = 0;
+  const float bottom = bin == kBins - 1 ? -3.4028235e38f : (float)((double)v.m - (bin + 1) * step - slack);
+  const uint32_t inv = (65536u + (v.seg_len >> 11) - 1) / (v.seg_len >> 11);   // segments are multiples of 2,048
+  uint32_t n = 0;   // the same in every lane
   for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int i) {
+    float most = g[0];
+#pragma unroll
+    for (int j = 1; j < V; ++j) most = fmaxf(most, g[j]);
+    if (!__any(most >= bottom)) return;
+    const uint32_t seg = ((uint32_t)(i >> 11) * inv) >> 16;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (g[j] <= top && g[j] >= bottom) {
-        const double y = log2_weight(g[j], v.m, v.r.c);
-        if (y >= kFloorLog2 && weight_bin(y) == bin) {
-          const uint32_t k = value_key(g[j]);
-          lo = k < lo ? k : lo;
-          hi = k > hi ? k : hi;
-          const uint32_t at = atomicAdd(&w.n, 1u);
-          if (at < RowWork<T, NT>::kList) {
-            w.list[at] = k;
-            w.list_seg[at] = (uint8_t)(i / v.seg_len);
-          }
+      const bool hit = g[j] <= top && g[j] >= bottom;
+      const uint64_t mask = __ballot(hit);
+      if (mask) {
+        const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        if (hit && at < kList) {
+          w.list[wave][at] = __float_as_uint(g[j]);
+          w.list_seg[wave][at] = (uint8_t)seg;
         }
+        n += (uint32_t)__popcll(mask);
       }
     }
   });
+  __syncthreads();
+  if (lane == 0) {
+    w.list_n[wave] = n < kList ? n : kList;
+    if (n > kList) w.listed = false;
+  }
+  __syncthreads();
+  uint32_t lo = 0xffffffffu, hi = 0;
+  const auto of_class = [&](float x) {
+    const double y = log2_weight(x, v.m, v.r.c);
+    if (!(y >= kFloorLog2) || weight_bin(y) != bin) return 0u;
+    const uint32_t k = value_key(x);
+    lo = k < lo ? k : lo;
+    hi = k > hi ? k : hi;
+    return k;
+  };
+  if (w.listed)
+    for (uint32_t i = lane; i < n; i += 64) w.list[wave][i] = of_class(__uint_as_float(w.list[wave][i]));
+  else
+    for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) of_class(g[j]);
+    });
   if (hi != 0) {
     atomicMin(&w.lo, lo);
     atomicMax(&w.hi, hi);
@@ -513,11 +572,11 @@ __device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<T, NT>
 
 // The value at which the count (or mass) counted from the top reaches `need`, inside the listed class.
 template <typename T, int NT>
-__device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<T, NT>& w, uint64_t above_mass, uint64_t above_count,
+__device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<NT>& w, uint64_t above_mass, uint64_t above_count,
                                       bool by_mass, uint64_t need) {
   constexpr int V = Vec16<T>::n;
   uint32_t lo = w.lo, hi = w.hi;
-  const uint32_t n = w.n;
+  const bool listed = w.listed;
   while (lo < hi) {   // at least 8 bits less each time
     int sh = 24 - __clz(hi - lo);
     if (sh < 0) sh = 0;
@@ -532,8 +591,8 @@ __device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<T, NT>& w, ui
                   (unsigned long long)weight_units(log2_weight(key_value(k), v.m, v.r.c), v.shift));
       }
     };
-    if (n <= RowWork<T, NT>::kList)
-      for (uint32_t i = threadIdx.x; i < n; i += NT) add(w.list[i]);
+    if (listed)
+      for_listed(w, [&](uint32_t k, int) { add(k); });
     else
       for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int) {
 #pragma unroll
@@ -557,7 +616,8 @@ __device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<T, NT>& w, ui
 
 // The cut of top-k and top-p, from the row's classes in w.mass, w.count.  `listed` is the class in w.list afterwards.
 template <typename T, int NT>
-__device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<T, NT>& w, uint64_t total, int& listed) {
+__device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<NT>& w, uint64_t total, int& listed) {
+  constexpr int kKeep = NT < kBins ? kBins / NT : 1;
   Cut cut{-INFINITY, 0, 0};
   uint64_t mass_k = total;
   listed = -1;
@@ -566,14 +626,19 @@ __device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<T, NT>& w, 
     const int bin = w.bin;
     if (bin >= 0) {   // else fewer than k have any weight
       const uint64_t am = w.above_mass, ac = w.above_count;
+      uint64_t keep[kKeep];   // the masses are needed again for top-p
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j) keep[j] = w.mass[(threadIdx.x + j * NT) % kBins];
       gather_class(v, w, bin);
       listed = bin;
       cut = refine(v, w, am, ac, false, (uint64_t)v.r.k);
       mass_k = cut.above + (uint64_t)cut.ties * weight_units(log2_weight(cut.value, v.m, v.r.c), v.shift);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kKeep; ++j) w.mass[(threadIdx.x + j * NT) % kBins] = keep[j];
     }
   }
   if (v.r.top_p < 1.f) {
-    if (listed >= 0) sum_classes(v, w);   // they were used up
     const uint64_t need = top_p_mass(v.r.top_p, mass_k);
     scan_classes(w, true, need);
     const int bin = w.bin < 0 ? 0 : w.bin;   // it is there: need <= total
@@ -588,20 +653,19 @@ __device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<T, NT>& w, 
 
 // The kept mass and the values at the cut of every segment -> w.seg_mass, w.seg_ties.
 template <typename T, int NT>
-__device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<T, NT>& w, const Cut& cut, int listed) {
+__device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<NT>& w, const Cut& cut, int listed) {
   constexpr int V = Vec16<T>::n, kWaves = NT / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const double y_cut = cut.value > -INFINITY ? log2_weight(cut.value, v.m, v.r.c) : kFloorLog2;
   const int bin = weight_bin(fmax(y_cut, v.r.ymin));   // above it everything is kept, below it nothing
   if (bin != listed) gather_class(v, w, bin);
   __syncthreads();
-  const uint32_t n = w.n;
-  if (n <= RowWork<T, NT>::kList) {
+  if (w.listed) {
     for (int s = wave; s < v.n_seg; s += kWaves) {
       uint64_t mass = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (64 * j + lane < bin) mass += v.seg_hist[(size_t)s * kBins + 64 * j + lane];
+        if (64 * j + lane < bin) mass += v.seg_hist[s * kBins + 64 * j + lane];
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
       if (lane == 0) {
@@ -610,15 +674,14 @@ __device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<T, NT>
       }
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += NT) {
-      const float x = key_value(w.list[i]);
-      const int s = w.list_seg[i];
+    for_listed(w, [&](uint32_t k, int s) {
+      const float x = key_value(k);
       const double y = log2_weight(x, v.m, v.r.c);
-      if (x == cut.value)
+      if (x == cut.value)   // x is NaN where there is none
         atomicAdd(&w.seg_ties[s], 1u);
       else if (x > cut.value && y >= v.r.ymin)
         atomicAdd((unsigned long long*)&w.seg_mass[s], (unsigned long long)weight_units(y, v.shift));
-    }
+    });
   } else {   // a flat row: over the whole of it again
     for (int s = wave; s < v.n_seg; s += kWaves) {
       const int begin = s * v.seg_len < v.A ? s * v.seg_len : v.A, end = begin + v.seg_len < v.A ? begin + v.seg_len : v.A;
@@ -650,7 +713,7 @@ __device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<T, NT>
 // Scans [begin, end) in index order for the first action whose running kept mass exceeds target; of the values at the cut
 // the first `left` are kept, each with `one` (0: none are).  True if it was there, else `seen` is the mass that was.
 template <typename T, int NT>
-__device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row, int begin,
+__device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row, int begin,
                                           int end, const Cut& cut, uint64_t one, uint32_t left, uint64_t target,
                                           uint64_t total, uint64_t& seen) {
   constexpr int V = Vec16<T>::n;
@@ -743,9 +806,9 @@ __device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<T, NT>& w
   return false;
 }
 
-// The draw of a filtered row, from its segments' classes (v.seg_hist) and, for top-k, the row's counts in w.count.
+// The draw of a filtered row, from its segments' classes.
 template <typename T, int NT>
-__device__ __forceinline__ void draw_filtered(const RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row) {
+__device__ __forceinline__ void draw_filtered(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row) {
   const uint64_t total = sum_classes(v, w);
   int listed;
   const Cut cut = find_cut(v, w, total, listed);
@@ -753,38 +816,51 @@ __device__ __forceinline__ void draw_filtered(const RowView<T>& v, RowWork<T, NT
   const double y_cut = cut.value > -INFINITY ? log2_weight(cut.value, v.m, v.r.c) : 0.0;
   // the values at the cut are kept if min_p keeps them
   const uint64_t one = cut.value > -INFINITY && y_cut >= v.r.ymin ? weight_units(y_cut, v.shift) : 0;
-  uint64_t mass = 0;
-  uint32_t left = one ? cut.ties : 0;
-  for (int s = 0; s < v.n_seg; ++s) {
-    const uint32_t t = w.seg_ties[s] < left ? w.seg_ties[s] : left;
-    mass += w.seg_mass[s] + (uint64_t)t * one;
-    left -= t;
+  // the first wave: a lane for each segment, its kept ties and its mass, their running sums, the draw's segment
+  static_assert(kMaxParts == 64, "a lane for each segment");
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    const uint32_t keep = one ? cut.ties : 0;
+    const uint32_t ties = lane < v.n_seg ? w.seg_ties[lane] : 0;
+    uint32_t tie_run = ties;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t o = __shfl_up(tie_run, off, 64);
+      if (lane >= off) tie_run += o;
+    }
+    const uint32_t tie_before = tie_run - ties;
+    const uint32_t left = tie_before < keep ? keep - tie_before : 0;
+    const uint64_t mass = (lane < v.n_seg ? w.seg_mass[lane] : 0) + (uint64_t)(ties < left ? ties : left) * one;
+    uint64_t run = mass;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint64_t o = __shfl_up(run, off, 64);
+      if (lane >= off) run += o;
+    }
+    const uint64_t target = draw_target(q.uniforms[row], __shfl(run, 63, 64));
+    if (run > target && run - mass <= target) {   // one lane
+      w.found = lane;
+      w.found_target = target - (run - mass);
+      w.lo = left;
+    }
   }
-  uint64_t target = draw_target(q.uniforms[row], mass);
-  left = one ? cut.ties : 0;
-  int s = 0;
-  for (; s < v.n_seg - 1; ++s) {
-    const uint32_t t = w.seg_ties[s] < left ? w.seg_ties[s] : left;
-    const uint64_t here = w.seg_mass[s] + (uint64_t)t * one;
-    if (here > target) break;
-    target -= here;
-    left -= t;
-  }
+  __syncthreads();
+  const int s = w.found;
+  const uint32_t left = w.lo;
+  const uint64_t target = w.found_target;
   const int begin = s * v.seg_len, end = begin + v.seg_len < v.A ? begin + v.seg_len : v.A;
   uint64_t seen;
   scan_draw(v, w, q, row, begin, end, cut, one, left, target, total, seen);
 }
 
-// The draw of a row without filters, from the sums of its pieces (n <= NT of them; v.m is not known yet).
+// The draw of a row without filters, from the sums of its n <= NT pieces.
 template <typename T, int NT>
-__device__ __forceinline__ void draw_pieces(RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row, const Pieces& p,
+__device__ __forceinline__ void draw_pieces(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row, const Pieces& p,
                                             int n) {
   constexpr int kLen = piece_length<T>();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x;
   const uint64_t raw = i < n ? p.mass[i] : 0;
   const float ref = i < n ? p.max[i] : -INFINITY;
-  bool bad = false;
-  v.m = group_max<NT>(ref, bad, w.red32);
   // the piece's mass relative to the row's maximum: exact where that is the piece's own, rounded to 53 bits elsewhere
   const double y = ref > -INFINITY ? log2_weight(ref, v.m, v.r.c) : -1e9;
   const uint64_t mass = y == 0.0 ? raw : y >= kFloorLog2 ? (uint64_t)rint((double)raw * exp2(y)) : 0;
@@ -824,7 +900,7 @@ __device__ __forceinline__ void draw_pieces(RowView<T>& v, RowWork<T, NT>& w, co
 
 // the largest logit, the first among equals
 template <typename T, int NT>
-__device__ __forceinline__ void draw_greedy(const RowView<T>& v, RowWork<T, NT>& w, const SampleArgs& q, int64_t row) {
+__device__ __forceinline__ void draw_greedy(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row) {
   constexpr int V = Vec16<T>::n;
   if (threadIdx.x == 0) w.found = 0x7fffffff;
   __syncthreads();
@@ -843,57 +919,131 @@ __device__ __forceinline__ void draw_greedy(const RowView<T>& v, RowWork<T, NT>&
 }
 
 // -1 for a row that has no distribution or nothing to choose from; true if it was one
-__device__ __forceinline__ bool no_draw(const SampleArgs& q, int64_t row, float m, bool bad) {
-  if (!bad && m > -INFINITY) return false;
+__device__ __forceinline__ bool no_draw(const SampleArgs& q, int64_t row, float m) {
+  if (m > -INFINITY) return false;
   if (threadIdx.x == 0) {
+    const bool bad = m != m;
     q.actions[row] = -1;
-    q.log_probs[row] = bad ? __builtin_nanf("") : 0.f;
+    q.log_probs[row] = bad ? m : 0.f;
     if (bad) *q.err = 1;
   }
   return true;
 }
 
-// `n` segments of a row: a multiple of every vector and of the loads in flight
-__host__ __device__ __forceinline__ int segment_length(int A, int n) { return ((A + n - 1) / n + 511) / 512 * 512; }
-
-// A workgroup per row.
+// the draw of a row whose maximum, pieces or classes are there
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void sample_row_kernel(const T* __restrict__ logits, int64_t stride, int A, SampleArgs q) {
-  __shared__ RowWork<T, NT> w;
-  constexpr int kWaves = NT / 64;
+__device__ __forceinline__ void draw_row(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row,
+                                         const Pieces& p) {
+  if (no_draw(q, row, v.m)) return;
+  if (v.r.greedy) draw_greedy(v, w, q, row);
+  else if (filtered(v.r)) draw_filtered(v, w, q, row);
+  else draw_pieces(v, w, q, row, p, (v.A + piece_length<T>() - 1) / piece_length<T>());
+}
+
+// Rows of up to kWaveRow actions: one wave each.
+constexpr int kWaveRow = 2048;
+
+template <typename T>
+__global__ __launch_bounds__(64) void sample_wave_kernel(const T* __restrict__ logits, int64_t stride, int A, SampleArgs q) {
+  constexpr int kPieces = kWaveRow / piece_length<T>();
+  __shared__ RowWork<64> w;
+  __shared__ uint64_t hist[kBins], piece_mass[kPieces];
+  __shared__ uint32_t count[kBins];
+  __shared__ float piece_max[kPieces];
   const int64_t row = blockIdx.x;
-  const int wave = threadIdx.x >> 6;
   RowView<T> v;
   v.x = logits + row * stride;
   v.A = A;
   v.r = row_settings(q, row);
   v.shift = q.shift;
-  bool bad;
-  if (!v.r.greedy && !filtered(v.r)) {
-    const int n = (A + piece_length<T>() - 1) / piece_length<T>();
-    const Pieces p{w.piece.mass, w.piece.max};
-    sum_pieces(v.x, A, v.r.c, v.shift, 0, n, wave, kWaves, p, bad);
-    // the largest piece's maximum decides whether there is anything to draw; the barriers order the pieces' sums too
-    __syncthreads();
-    float m = (int)threadIdx.x < n ? p.max[threadIdx.x] : -INFINITY;
-    m = group_max<NT>(m, bad, w.red32);
-    if (no_draw(q, row, m, bad)) return;
-    draw_pieces(v, w, q, row, p, n);
-    return;
-  }
-  v.m = part_max<T, NT>(v.x, 0, A, bad);
-  v.m = group_max<NT>(v.m, bad, w.red32);
-  if (no_draw(q, row, v.m, bad)) return;
-  if (v.r.greedy) return draw_greedy(v, w, q, row);
-  v.n_seg = kWaves;
-  v.seg_len = segment_length(A, kWaves);
-  v.seg_hist = &w.wave_mass[0][0];
-  for (int i = threadIdx.x; i < kWaves * kBins; i += NT) (&w.wave_mass[0][0])[i] = 0;
-  for (int i = threadIdx.x; i < kBins; i += NT) w.count[i] = 0;
+  v.n_seg = 1;
+  v.seg_len = kWaveRow;
+  v.seg_hist = hist;
+  v.seg_count = count;
+  const Pieces p{piece_mass, piece_max};
+  const bool hists = filtered(v.r);
+  sum_pieces(v.x, A, v.r.c, v.shift, 0, (A + piece_length<T>() - 1) / piece_length<T>(), 0, 1, p, !hists && !v.r.greedy);
   __syncthreads();
-  const int begin = wave * v.seg_len < A ? wave * v.seg_len : A, end = begin + v.seg_len < A ? begin + v.seg_len : A;
-  add_classes(v.x, begin, end, v.m, v.r, v.shift, w.wave_mass[wave], w.count);
-  draw_filtered(v, w, q, row);
+  v.m = row_max<T, 64>(p, A, w.red32);
+  if (hists && v.m > -INFINITY) {
+    for (int i = threadIdx.x; i < kBins; i += 64) { hist[i] = 0; count[i] = 0; }
+    __syncthreads();
+    add_classes<T, 64>(v.x, 0, A, v.m, v.r, v.shift, hist, count);
+    __syncthreads();
+  }
+  draw_row(v, w, q, row, p);
+}
+
+// Longer rows: how a batch is cut.  What a row leaves in the workspace: its pieces' masses and maxima and, where it has
+// filters, its segments' classes.
+struct SamplePlan {
+  int n_seg, seg_len, n_piece;
+  int64_t group;                         // rows that go through the three launches together
+  uint64_t* piece_mass;                  // [B][n_piece]
+  uint64_t* seg_hist;                    // [group][n_seg][kBins]
+  uint32_t* seg_count;                   // [group][n_seg][kBins]
+  float* piece_max;                      // [B][n_piece]
+};
+
+constexpr int kPartThreads = 256;
+
+// a workgroup per segment: the pieces' maxima, and their masses where that is all a row needs
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_pieces_kernel(const T* __restrict__ logits, int64_t stride, int A,
+                                                                     SampleArgs q, SamplePlan plan, int64_t row0) {
+  const int64_t row = row0 + blockIdx.x / plan.n_seg;
+  const int seg = blockIdx.x % plan.n_seg;
+  const Row r = row_settings(q, row);
+  const int per = plan.seg_len / piece_length<T>(), n = (A + piece_length<T>() - 1) / piece_length<T>();
+  const int first = seg * per, last = first + per < n ? first + per : n;
+  const Pieces p{plan.piece_mass + row * plan.n_piece, plan.piece_max + row * plan.n_piece};
+  sum_pieces(logits + row * stride, A, r.c, q.shift, first, last, threadIdx.x >> 6, kPartThreads / 64, p,
+             !r.greedy && !filtered(r));
+}
+
+// a workgroup per segment: its classes, where the row has filters
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_classes_kernel(const T* __restrict__ logits, int64_t stride, int A,
+                                                                      SampleArgs q, SamplePlan plan, int64_t row0) {
+  __shared__ uint64_t hist[kBins];
+  __shared__ uint32_t count[kBins], red[kPartThreads / 64];
+  const int64_t row = row0 + blockIdx.x / plan.n_seg;
+  const int seg = blockIdx.x % plan.n_seg;
+  const Row r = row_settings(q, row);
+  if (!filtered(r)) return;
+  const Pieces p{nullptr, plan.piece_max + row * plan.n_piece};
+  const float m = row_max<T, kPartThreads>(p, A, red);
+  if (!(m > -INFINITY)) return;
+  static_assert(kPartThreads == kBins, "a thread for each class");
+  hist[threadIdx.x] = 0;
+  count[threadIdx.x] = 0;
+  __syncthreads();
+  const int begin = seg * plan.seg_len, end = begin + plan.seg_len < A ? begin + plan.seg_len : A;
+  add_classes<T, kPartThreads>(logits + row * stride, begin, end, m, r, q.shift, hist, count);
+  __syncthreads();
+  const int64_t at = ((row - row0) * plan.n_seg + seg) * kBins + threadIdx.x;
+  plan.seg_hist[at] = hist[threadIdx.x];
+  if (r.k > 0) plan.seg_count[at] = count[threadIdx.x];
+}
+
+// a workgroup per row: the rest
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void sample_finish_kernel(const T* __restrict__ logits, int64_t stride, int A, SampleArgs q,
+                                                           SamplePlan plan, int64_t row0) {
+  __shared__ RowWork<NT> w;
+  const int64_t row = row0 + blockIdx.x;
+  RowView<T> v;
+  v.x = logits + row * stride;
+  v.A = A;
+  v.r = row_settings(q, row);
+  v.shift = q.shift;
+  v.n_seg = plan.n_seg;
+  v.seg_len = plan.seg_len;
+  v.seg_hist = plan.seg_hist + blockIdx.x * (int64_t)plan.n_seg * kBins;
+  v.seg_count = plan.seg_count + blockIdx.x * (int64_t)plan.n_seg * kBins;
+  const Pieces p{plan.piece_mass + row * plan.n_piece, plan.piece_max + row * plan.n_piece};
+  v.m = row_max<T, NT>(p, A, w.red32);
+  draw_row(v, w, q, row, p);
 }
 
 static inline int sample_shift(int64_t A) {
@@ -902,8 +1052,40 @@ static inline int sample_shift(int64_t A) {
   return 62 - bits < 51 ? 62 - bits : 51;
 }
 
+static SamplePlan sample_plan(int64_t B, int64_t A, void* workspace) {
+  constexpr int64_t kPiece = piece_length<float>();   // the shorter ones
+  SamplePlan p;
+  p.group = ((int64_t)256 << 20) / A;                 // 100 MB of classes
+  if (p.group < 1) p.group = 1;
+  if (p.group > B) p.group = B;
+  // segments of about 8,192 actions (the last pass scans one of them), of fewer where the rows are few
+  int64_t n = (A + 8191) / 8192;
+  const int64_t few = 2048 / p.group, most = A / 4096;
+  if (n < few && n < most) n = few < most ? few : most;
+  if (n > kMaxParts) n = kMaxParts;
+  p.seg_len = (int)(((A + n - 1) / n + 2047) / 2048 * 2048);
+  p.n_seg = (int)((A + p.seg_len - 1) / p.seg_len);
+  p.n_piece = (int)((A + kPiece - 1) / kPiece);
+  char* at = (char*)workspace;
+  p.piece_mass = (uint64_t*)at;
+  at += B * p.n_piece * 8;
+  p.seg_hist = (uint64_t*)at;
+  at += p.group * p.n_seg * kBins * 8;
+  p.seg_count = (uint32_t*)at;
+  at += p.group * p.n_seg * kBins * 4;
+  p.piece_max = (float*)at;
+  return p;
+}
+
+static size_t sample_workspace(int64_t B, int64_t A) {
+  if (B <= 0 || A <= kWaveRow) return 0;
+  const SamplePlan p = sample_plan(B, A, nullptr);
+  return (size_t)B * p.n_piece * 12 + (size_t)p.group * p.n_seg * kBins * 12;
+}
+
 template <typename T>
-static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, const SampleArgs& q, hipStream_t s) {
+static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, const SampleArgs& q, void* workspace,
+                      hipStream_t s) {
   if (A <= 64) {
     const int lanes = A <= 8 ? 8 : A <= 16 ? 16 : A <= 32 ? 32 : 64;
     const int grid = (int)((B * lanes + 255) / 256);
@@ -911,21 +1093,43 @@ static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, con
     else if (lanes == 16) sample_small_kernel<T, 16><<<grid, 256, 0, s>>>(logits, stride, B, (int)A, q);
     else if (lanes == 32) sample_small_kernel<T, 32><<<grid, 256, 0, s>>>(logits, stride, B, (int)A, q);
     else sample_small_kernel<T, 64><<<grid, 256, 0, s>>>(logits, stride, B, (int)A, q);
-  } else if (A <= 2048) {
-    sample_row_kernel<T, 64><<<(int)B, 64, 0, s>>>(logits, stride, (int)A, q);
-  } else if (A <= 16384) {
-    sample_row_kernel<T, 256><<<(int)B, 256, 0, s>>>(logits, stride, (int)A, q);
-  } else {
-    sample_row_kernel<T, 1024><<<(int)B, 1024, 0, s>>>(logits, stride, (int)A, q);
+    return check_launch();
   }
-  return check_launch();
+  if (A <= kWaveRow) {
+    sample_wave_kernel<T><<<(int)B, 64, 0, s>>>(logits, stride, (int)A, q);
+    return check_launch();
+  }
+  const SamplePlan p = sample_plan(B, A, workspace);
+  const bool per_row = q.temperature || q.top_k || q.top_p || q.min_p;
+  const bool greedy = !per_row && q.temperature_s == 0.f;
+  const bool filters = per_row || (!greedy && (q.top_k_s > 0 || q.top_p_s < 1.f || q.min_p_s > 0.f));
+  const int64_t group = filters ? p.group : B;
+  for (int64_t row0 = 0; row0 < B; row0 += group) {
+    const int64_t rows = row0 + group < B ? group : B - row0;
+    const int parts = (int)(rows * p.n_seg);
+    sample_pieces_kernel<T><<<parts, kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    if (int rc = check_launch()) return rc;
+    if (filters) {
+      sample_classes_kernel<T><<<parts, kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
+      if (int rc = check_launch()) return rc;
+    }
+    // all the threads a workgroup can have for a pass over the row; where there is none, four times as many rows side by side
+    if (filters || greedy || rows < 512 || A > 256 * piece_length<T>())
+      sample_finish_kernel<T, 1024><<<(int)rows, 1024, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    else
+      sample_finish_kernel<T, 256><<<(int)rows, 256, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    if (int rc = check_launch()) return rc;
+  }
+  return PARLHIP_OK;
 }
 
 }  // namespace parlhip
 
 using namespace parlhip;
 
-PARLHIP_EXPORT size_t parlhip_logits_sample_workspace_bytes(int64_t B, int64_t A) { return 0; }
+PARLHIP_EXPORT size_t parlhip_logits_sample_workspace_bytes(int64_t B, int64_t A) {
+  return A < 1 || A > kSampleMaxActions ? 0 : sample_workspace(B, A);
+}
 
 PARLHIP_EXPORT int parlhip_logits_sample(const void* logits, int dtype, int64_t row_stride, const double* uniforms,
                                          const float* temperature, const int32_t* top_k, const float* top_p,
@@ -934,18 +1138,22 @@ PARLHIP_EXPORT int parlhip_logits_sample(const void* logits, int dtype, int64_t 
                                          void* workspace, size_t workspace_bytes, parlhip_stream_t stream) {
   if (B < 0 || A < 1 || row_stride < A) return PARLHIP_EINVAL;
   if (dtype != PARLHIP_F32 && dtype != PARLHIP_BF16 && dtype != PARLHIP_F16) return PARLHIP_ENOSUP;
-  if (A > kSampleMaxActions || B > 0xffffffffLL / 1024) return PARLHIP_ENOSUP;   // one launch's threads
+  // one launch's threads: 64 for a row at most, or 256 for each of its segments
+  if (A > kSampleMaxActions || B > 0xffffffffLL / (A <= kWaveRow ? 64 : 256 * kMaxParts)) return PARLHIP_ENOSUP;
   if (!temperature && !(temperature_all >= 0.f && temperature_all < INFINITY)) return PARLHIP_EINVAL;
   if (!top_p && !(top_p_all >= 0.f)) return PARLHIP_EINVAL;
   if (!min_p && !(min_p_all >= 0.f && min_p_all <= 1.f)) return PARLHIP_EINVAL;
   if (B == 0) return PARLHIP_OK;
   if (!logits || !uniforms || !actions || !log_probs) return PARLHIP_EINVAL;
   if (reinterpret_cast<uintptr_t>(logits) & (dtype == PARLHIP_F32 ? 3 : 1)) return PARLHIP_EINVAL;
+  const size_t need = sample_workspace(B, A);
+  if (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 7))) return PARLHIP_EINVAL;
+  if (workspace_bytes < need) return PARLHIP_ENOMEM;
   SampleArgs q{uniforms, temperature, top_k, top_p, min_p, temperature_all, top_p_all, min_p_all, top_k_all,
                actions, log_probs, device_error_flag(), sample_shift(A)};
   if (!q.err) return PARLHIP_ELAUNCH;
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == PARLHIP_F32) return sample_run((const float*)logits, row_stride, B, A, q, s);
-  if (dtype == PARLHIP_BF16) return sample_run((const bf16_t*)logits, row_stride, B, A, q, s);
-  return sample_run((const f16_t*)logits, row_stride, B, A, q, s);
+  if (dtype == PARLHIP_F32) return sample_run((const float*)logits, row_stride, B, A, q, workspace, s);
+  if (dtype == PARLHIP_BF16) return sample_run((const bf16_t*)logits, row_stride, B, A, q, workspace, s);
+  return sample_run((const f16_t*)logits, row_stride, B, A, q, workspace, s);
 }

@@ -31,6 +31,22 @@ def test_sample_arguments(lib):
     assert _sample(lib, B=0, logits=None, u=None, a=None, lp=None) == 0
 
 
+def test_sample_workspace(lib):
+    f = lib.parlhip_logits_sample_workspace_bytes
+    for A in (1, 64, 65, 2048):
+        assert f(1000, A) == 0
+    assert f(0, 100000) == 0 and f(5, 0) == 0 and f(5, (1 << 20) + 1) == 0
+    for A in (2049, 3000, 4095, 4096, 4097, 8191, 8193, 16385, 50000, 131072, 262143, 1 << 20):
+        for B in (1, 2, 63, 300, 5000, 262143):
+            n = f(B, A)
+            # the pieces' sums of every row, and no more than the logits themselves behind that
+            assert B * (A // 1024) * 12 <= n <= B * (A // 1024 + 1) * 12 + 4 * B * A + (1 << 20), (A, B)
+    need = f(3, 5000)
+    assert _sample(lib, B=3, A=5000, stride=5000, wsb=need - 1) == NOMEM
+    assert _sample(lib, B=3, A=5000, stride=5000, ws=None) == INVALID
+    assert _sample(lib, B=3, A=5000, stride=5000, ws=20) == INVALID
+
+
 def test_log_prob_arguments(lib):
     def f(x=16, dtype=0, stride=8, a=16, lp=16, h=16, st=16, N=2, A=8, T=1.0, ws=16, wsb=1 << 40):
         return lib.parlhip_logits_log_prob(x, dtype, stride, a, lp, h, st, N, A, T, ws, wsb, None)
