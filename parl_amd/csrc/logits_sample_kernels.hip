@@ -247,7 +247,7 @@ struct Pieces {          // of one row
 template <int NT>
 struct RowWork {
   static constexpr int kWaves = NT / 64;
-  static constexpr int kList = NT == 64 ? 1024 : 512;   // of each wave
+  static constexpr int kList = NT == 1024 ? 512 : 1024;   // of each wave
   uint64_t mass[kBins];                  // of the row, or of the class that is being taken apart
   uint32_t count[kBins];
   uint32_t list[kWaves][kList];          // the values (keys; 0: none) of a class and the segments that they are in
@@ -1113,9 +1113,12 @@ static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, con
       sample_classes_kernel<T><<<parts, kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
       if (int rc = check_launch()) return rc;
     }
-    // all the threads a workgroup can have for a pass over the row; where there is none, four times as many rows side by side
-    if (filters || greedy || rows < 512 || A > 256 * piece_length<T>())
+    // a thread for each piece of a row; else smaller workgroups, more rows side by side, where the rows are many
+    const int pieces = (int)((A + piece_length<T>() - 1) / piece_length<T>());
+    if (pieces > 512)
       sample_finish_kernel<T, 1024><<<(int)rows, 1024, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    else if (rows < 512 || pieces > 256)
+      sample_finish_kernel<T, 512><<<(int)rows, 512, 0, s>>>(logits, stride, (int)A, q, p, row0);
     else
       sample_finish_kernel<T, 256><<<(int)rows, 256, 0, s>>>(logits, stride, (int)A, q, p, row0);
     if (int rc = check_launch()) return rc;
