@@ -180,10 +180,11 @@ __global__ __launch_bounds__(NT) void logprob_row_kernel(const T* __restrict__ l
   const T* x = logits + row * stride;
   const int64_t begin = p * part;
   const int64_t end = begin + part < A ? begin + part : A;
-  const Stat st = part_stat<T, NT>(x, begin, end, c, lds);
+  const int64_t a = row_action(actions, row, A, err);
+  const Stat st = a >= 0 ? part_stat<T, NT>(x, begin, end, c, lds) : stat_empty();   // no decision: nothing to read
   if (threadIdx.x != 0) return;
   if (n_parts == 1)
-    row_finish(st, x, row_action(actions, row, A, err), row, inv_t, log_probs, entropies, stats);
+    row_finish(st, x, a, row, inv_t, log_probs, entropies, stats);
   else
     parts[blockIdx.x] = st;
 }
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(256) void logprob_small_grad_kernel(
   }
 }
 
-// One workgroup per (row, part of the row).
+// One workgroup per (row, part of the row), with two loads of each thread in flight.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void logprob_row_grad_kernel(
     const T* __restrict__ logits, int64_t stride, const int64_t* __restrict__ actions, const float2* __restrict__ stats,
@@ -268,25 +269,35 @@ __global__ __launch_bounds__(NT) void logprob_row_grad_kernel(
   const T* x = logits + row * stride;
   T* o = grad + row * A;
   const GradRow r = grad_row(actions, stats, entropies, g_logp, g_ent, row, A, inv_t);
-  for (int64_t i = begin + (int64_t)threadIdx.x * V; i < end; i += (int64_t)NT * V) {
-    if (i + V <= end) {
-      Vec16<T> v, w;
-      float f[V];
-      if (r.live) {
-        v.load(x + i);
-        v.unpack(f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = grad_at(r, f[j], i + j, c);
-      } else {   // no decision: nothing to read
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = 0.f;
-      }
-      w.pack(f);
-      w.store(o + i);
-    } else {
-      for (int64_t j = i; j < end; ++j) from_f32(r.live ? grad_at(r, to_f32(x[j]), j, c) : 0.f, o[j]);
-    }
+  int64_t i = begin + (int64_t)threadIdx.x * V;
+  if (!r.live) {   // no decision: nothing to read
+    const Vec16<T> zero{u32x4{0, 0, 0, 0}};
+    for (; i + V <= end; i += (int64_t)NT * V) zero.store(o + i);
+    for (; i < end; ++i) from_f32(0.f, o[i]);   // at most one thread has a rest of less than V
+    return;
   }
+  const auto put = [&](const Vec16<T>& v, int64_t at) {
+    float f[V];
+    v.unpack(f);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = grad_at(r, f[j], at + j, c);
+    Vec16<T> w;
+    w.pack(f);
+    w.store(o + at);
+  };
+  for (; i + (int64_t)NT * V + V <= end; i += (int64_t)2 * NT * V) {
+    Vec16<T> v[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) v[u].load(x + i + (int64_t)u * NT * V);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) put(v[u], i + (int64_t)u * NT * V);
+  }
+  for (; i + V <= end; i += (int64_t)NT * V) {
+    Vec16<T> v;
+    v.load(x + i);
+    put(v, i);
+  }
+  for (; i < end; ++i) from_f32(grad_at(r, to_f32(x[i]), i, c), o[i]);
 }
 
 // How the rows are cut: few long rows are split over several workgroups so that about 1,024 of them (four per CU) run.
@@ -309,6 +320,9 @@ static LogprobPlan logprob_plan(int64_t N, int64_t A) {
 
 constexpr int64_t kMaxSmall = 512;      // 64 lanes x 8 logits
 constexpr int64_t kMaxWaveRow = 4096;   // one wave per row up to here
+// Above, the more threads the longer the stretch of a row that is read at a time, and the fewer rows side by side: 4,096 rows
+// of 131,072 bf16 take 613 / 594 / 579 us with 256 / 512 / 1,024 threads (both passes), 2,048 of 32,003 take 92 / 90 / 105.
+constexpr int64_t kRow512 = 16384, kRow1024 = 65536;
 
 template <typename T>
 static int logprob_forward(const T* logits, int64_t stride, const int64_t* actions, float* log_probs, float* entropies,
@@ -332,9 +346,15 @@ static int logprob_forward(const T* logits, int64_t stride, const int64_t* actio
   if (A <= kMaxWaveRow)
     logprob_row_kernel<T, 64><<<grid, 64, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts, N, A,
                                                   p.n_parts, p.part, c, inv_t, err);
+  else if (A < kRow512)
+    logprob_row_kernel<T, 256><<<grid, 256, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts,
+        N, A, p.n_parts, p.part, c, inv_t, err);
+  else if (A < kRow1024)
+    logprob_row_kernel<T, 512><<<grid, 512, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts,
+        N, A, p.n_parts, p.part, c, inv_t, err);
   else
-    logprob_row_kernel<T, 256><<<grid, 256, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts, N, A,
-                                                    p.n_parts, p.part, c, inv_t, err);
+    logprob_row_kernel<T, 1024><<<grid, 1024, 0, s>>>(logits, stride, actions, log_probs, entropies, stats,
+        parts, N, A, p.n_parts, p.part, c, inv_t, err);
   int rc = check_launch();
   if (rc || p.n_parts == 1) return rc;
   logprob_join_kernel<T><<<(int)N, 64, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts, A, p.n_parts, c, inv_t, err);
@@ -362,9 +382,15 @@ static int logprob_backward(const T* logits, int64_t stride, const int64_t* acti
   if (A <= kMaxWaveRow)
     logprob_row_grad_kernel<T, 64><<<grid, 64, 0, s>>>(logits, stride, actions, stats, entropies, g_logp, g_ent, grad, A,
                                                        p.n_parts, p.part, c, inv_t);
+  else if (A < kRow512)
+    logprob_row_grad_kernel<T, 256><<<grid, 256, 0, s>>>(logits, stride, actions, stats, entropies, g_logp,
+        g_ent, grad, A, p.n_parts, p.part, c, inv_t);
+  else if (A < kRow1024)
+    logprob_row_grad_kernel<T, 512><<<grid, 512, 0, s>>>(logits, stride, actions, stats, entropies, g_logp,
+        g_ent, grad, A, p.n_parts, p.part, c, inv_t);
   else
-    logprob_row_grad_kernel<T, 256><<<grid, 256, 0, s>>>(logits, stride, actions, stats, entropies, g_logp, g_ent, grad, A,
-                                                         p.n_parts, p.part, c, inv_t);
+    logprob_row_grad_kernel<T, 1024><<<grid, 1024, 0, s>>>(logits, stride, actions, stats, entropies, g_logp,
+        g_ent, grad, A, p.n_parts, p.part, c, inv_t);
   return check_launch();
 }
 

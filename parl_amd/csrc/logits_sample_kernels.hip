@@ -31,6 +31,8 @@ namespace parlhip {
 constexpr int64_t kSampleMaxActions = (int64_t)1 << 20;
 constexpr double kFloorLog2 = -42.0;     // weights under 2^-42 are 0
 constexpr int kBins = 256;
+constexpr double kPerHalving = 6.0;
+constexpr int kLastBin = 252;            // 42 halvings
 constexpr int kMaxParts = 64;       // of a row that several workgroups share
 
 struct SampleArgs {
@@ -88,31 +90,32 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // log2 of a weight; 0 at the maximum
 __device__ __forceinline__ double log2_weight(float x, float m, double c) { return ((double)x - (double)m) * c; }
 
-// 2^y in units of 2^-shift, rounded to nearest, 0 where y < -42; y <= 0, shift <= 51.  2^r = 1 + r q(r) on |r| <= 1/2 with
-// q the interpolation of (2^r - 1) / r at eight Chebyshev nodes: relative error 2e-12, and 2^0 is 1.  Adding 2^52 to a
-// number below it leaves its nearest integer in the low bits.  No branch: the weights of a load are formed side by side.
-// Some 75 cycles of the vector unit for 64 weights; float64 runs at float32's rate here.
-__device__ __forceinline__ uint64_t weight_units(double y, int shift) {
-  const double n = rint(y), r = y - n;
-  double p = 0x1.63b2d7971923fp-20;
-  p = __builtin_fma(p, r, 0x1.00c0e4e15189cp-16);
-  p = __builtin_fma(p, r, 0x1.4308c7183d6a2p-13);
-  p = __builtin_fma(p, r, 0x1.5d877598350dep-10);
-  p = __builtin_fma(p, r, 0x1.3b2ab70ad2565p-7);
-  p = __builtin_fma(p, r, 0x1.c6b08da70cce3p-5);
-  p = __builtin_fma(p, r, 0x1.ebfbdff82a734p-3);
-  p = __builtin_fma(p, r, 0x1.62e42fef9cc69p-1);
+// 2^y in units of 2^-shift, rounded to nearest, 0 where y < -42, plus kUnitsBase; y <= 0, shift <= 51.  2^r = 1 + r q(r) on
+// |r| <= 1/2 with q the interpolation of (2^r - 1) / r at seven Chebyshev nodes: relative error 1.1e-10, and 2^0 is 1.
+// (The error is a function of r alone, so most of it cancels between a running sum and the whole: over 131,072 actions a
+// border moves by some 1e-13 of the mass.)  Adding 2^52 to a number below it leaves its nearest integer in the low bits.  No
+// branch: the weights of a load are formed side by side, 15 instructions of the vector unit each; float64 runs at
+// float32's rate here.
+constexpr uint64_t kUnitsBase = 0x4330000000000000ULL;
+__device__ __forceinline__ uint64_t weight_bits(double y, int shift) {
+  y = fmax(y, -1000.0);   // -inf: no NaN below
+  // adding 1.5 * 2^52 rounds to an integer, which then is the low word: n + shift + 1023, the exponent of the weight
+  const double magic = 0x1.8p52 + (shift + 1023), t = y + magic, r = y - (t - magic);
+  double p = 0x1.00a581594758ep-16;
+  p = __builtin_fma(p, r, 0x1.443fffc90db59p-13);
+  p = __builtin_fma(p, r, 0x1.5d879ead06a82p-10);
+  p = __builtin_fma(p, r, 0x1.3b2a1b7152befp-7);
+  p = __builtin_fma(p, r, 0x1.c6b08d883dca1p-5);
+  p = __builtin_fma(p, r, 0x1.ebfbe045f4d3cp-3);
+  p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);
   p = __builtin_fma(p, r, 1.0);
-  const double scale = __hiloint2double((int)((uint32_t)((int)n + shift + 1023) << 20), 0);   // 2^(n + shift)
-  const uint64_t bits = (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
-  return y >= kFloorLog2 ? bits & 0xfffffffffffffULL : 0;
+  const double scale = __hiloint2double(y >= kFloorLog2 ? __double2loint(t) << 20 : 0, 0);   // 2^(n + shift)
+  return (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
 }
+__device__ __forceinline__ uint64_t weight_units(double y, int shift) { return weight_bits(y, shift) - kUnitsBase; }
 
-// the class of a weight: 0 for the largest, 255 for those just above 2^-42
-__device__ __forceinline__ int weight_bin(double y) {
-  const int b = (int)(y * (-(double)kBins / 42.0));
-  return b < kBins - 1 ? b : kBins - 1;
-}
+// the class of a weight: six for each halving, 0 for the largest, 252 for 2^-42
+__device__ __forceinline__ int weight_bin(double y) { return (int)(y * -kPerHalving); }
 
 // u * mass rounded down to whole units; u is a multiple of 2^-53, so this is exact: the draw is the first action whose
 // running mass exceeds it, and there always is one
@@ -311,6 +314,10 @@ __device__ __forceinline__ float group_max(float m, uint32_t* lds) {
   return m;
 }
 
+__device__ __forceinline__ float maximum3(float a, float b, float c) {   // NaN if any is
+  return __builtin_elementwise_maximum(a, __builtin_elementwise_maximum(b, c));
+}
+
 // The pieces [first, last) of a row, one after the other by each of the waves `wave` of `waves`: their maxima and, with
 // SUM, their masses relative to these.
 template <typename T>
@@ -336,24 +343,20 @@ __device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, doubl
         raw[a].pack(g);   // exact: they came from this type
       }
     }
-    float m = -INFINITY;
-    bool bad = false;
+    float m = -INFINITY;   // a NaN stays
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float g = raw[a].get(j);
-        bad |= !(g < INFINITY);
-        m = fmaxf(m, g);
-      }
-    m = group_max<64>(bad ? __builtin_nanf("") : m, nullptr);
+      for (int j = 0; j < V; j += 2) m = maximum3(m, raw[a].get(j), raw[a].get(j + 1));
+    m = group_max<64>(m < INFINITY ? m : __builtin_nanf(""), nullptr);
     if (sum) {
       uint64_t mass = 0;
       if (m > -INFINITY) {
 #pragma unroll
         for (int a = 0; a < 4; ++a)
 #pragma unroll
-          for (int j = 0; j < V; ++j) mass += weight_units(log2_weight(raw[a].get(j), m, c), shift);
+          for (int j = 0; j < V; ++j) mass += weight_bits(log2_weight(raw[a].get(j), m, c), shift);
+        mass -= 4 * V * kUnitsBase;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
       }
@@ -392,7 +395,7 @@ __device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, 
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (u[j]) {
+      if (y[j] >= kFloorLog2) {
         const int b = weight_bin(y[j]);
         atomicAdd((unsigned long long*)&mass[b], (unsigned long long)u[j]);
         if (r.k > 0) atomicAdd(&count[b], 1u);
@@ -516,9 +519,9 @@ __device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<NT>& w
   // A little more than the class' range: one comparison for a load's values together where they are all below it, else two
   // for each.  A wave appends what it finds to a list of its own; whether it is of the class is seen afterwards, on
   // the list (float64 in this loop would run for every second load of a wave).
-  const double step = 42.0 / kBins / v.r.c, slack = 1e-6 * (fabs((double)v.m) + (bin + 1) * step) + 1e-37;
+  const double step = 1.0 / kPerHalving / v.r.c, slack = 1e-6 * (fabs((double)v.m) + (bin + 1) * step) + 1e-37;
   const float top = (float)((double)v.m - bin * step + slack);
-  const float bottom = bin == kBins - 1 ? -3.4028235e38f : (float)((double)v.m - (bin + 1) * step - slack);
+  const float bottom = bin == kLastBin ? -3.4028235e38f : (float)((double)v.m - (bin + 1) * step - slack);
   const uint32_t inv = (65536u + (v.seg_len >> 11) - 1) / (v.seg_len >> 11);   // segments are multiples of 2,048
   uint32_t n = 0;   // the same in every lane
   for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int i) {
