@@ -96,18 +96,25 @@ __device__ __forceinline__ double log2_weight(float x, float m, double c) { retu
 // border moves by some 1e-13 of the mass.)  Adding 2^52 to a number below it leaves its nearest integer in the low bits.  No
 // branch: the weights of a load are formed side by side, 15 instructions of the vector unit each; float64 runs at
 // float32's rate here.
+// a b + c with c in scalar registers: left to itself the compiler copies the constant into the result's registers first, one
+// instruction more for every step
+__device__ __forceinline__ double fma_const(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
+}
 constexpr uint64_t kUnitsBase = 0x4330000000000000ULL;
 __device__ __forceinline__ uint64_t weight_bits(double y, int shift) {
   y = fmax(y, -1000.0);   // -inf: no NaN below
   // adding 1.5 * 2^52 rounds to an integer, which then is the low word: n + shift + 1023, the exponent of the weight
   const double magic = 0x1.8p52 + (shift + 1023), t = y + magic, r = y - (t - magic);
   double p = 0x1.00a581594758ep-16;
-  p = __builtin_fma(p, r, 0x1.443fffc90db59p-13);
-  p = __builtin_fma(p, r, 0x1.5d879ead06a82p-10);
-  p = __builtin_fma(p, r, 0x1.3b2a1b7152befp-7);
-  p = __builtin_fma(p, r, 0x1.c6b08d883dca1p-5);
-  p = __builtin_fma(p, r, 0x1.ebfbe045f4d3cp-3);
-  p = __builtin_fma(p, r, 0x1.62e42fefa39efp-1);
+  p = fma_const(p, r, 0x1.443fffc90db59p-13);
+  p = fma_const(p, r, 0x1.5d879ead06a82p-10);
+  p = fma_const(p, r, 0x1.3b2a1b7152befp-7);
+  p = fma_const(p, r, 0x1.c6b08d883dca1p-5);
+  p = fma_const(p, r, 0x1.ebfbe045f4d3cp-3);
+  p = fma_const(p, r, 0x1.62e42fefa39efp-1);
   p = __builtin_fma(p, r, 1.0);
   const double scale = __hiloint2double(y >= kFloorLog2 ? __double2loint(t) << 20 : 0, 0);   // 2^(n + shift)
   return (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
