@@ -35,6 +35,33 @@ constexpr double kPerHalving = 6.0;
 constexpr int kLastBin = 252;            // 42 halvings
 constexpr int kMaxParts = 64;       // of a row that several workgroups share
 
+// Running sums over the lanes of a wave, by the data-parallel moves of the vector unit (a shuffle goes through LDS and takes
+// several times as long): within rows of 16 lanes, then the rows' last lanes into the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_move(uint32_t x) {   // 0 where there is no source
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lane_move(uint64_t x) {
+  return (uint64_t)lane_move<CTRL, ROWS>((uint32_t)x) | (uint64_t)lane_move<CTRL, ROWS>((uint32_t)(x >> 32)) << 32;
+}
+template <typename X>
+__device__ __forceinline__ X wave_scan(X x) {
+  x += lane_move<0x111, 0xf>(x);   // from 1, 2, 4, 8 lanes below, inside a row
+  x += lane_move<0x112, 0xf>(x);
+  x += lane_move<0x114, 0xf>(x);
+  x += lane_move<0x118, 0xf>(x);
+  x += lane_move<0x142, 0xa>(x);   // lane 15 of the row below, into rows 1 and 3
+  x += lane_move<0x143, 0xc>(x);   // lane 31, into rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
+  return (uint64_t)last_lane((uint32_t)x) | (uint64_t)last_lane((uint32_t)(x >> 32)) << 32;
+}
+template <typename X>
+__device__ __forceinline__ X wave_total(X x) { return last_lane(wave_scan(x)); }
+
 struct SampleArgs {
   const double* uniforms;
   const float* temperature;   // per row, or NULL: the scalar behind it
@@ -287,12 +314,13 @@ struct RowView {
   int n_seg, seg_len;                    // segment s: [s * seg_len, ...); seg_len is a multiple of every vector
   const uint64_t* seg_hist;              // [n_seg][kBins]: masses of the classes
   const uint32_t* seg_count;             // and counts
+  const uint32_t* seg_first;             // [n_seg][kBins], or NULL: where a class begins among the segment's values,
+  const float* values;                   // [n_seg][seg_len], which then are in the order of their classes
 };
 
 template <typename X, int NT>
 __device__ __forceinline__ X group_sum(X v, X* lds) {   // every thread gets the sum
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+  v = wave_total(v);
   if constexpr (NT > 64) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -364,8 +392,7 @@ __device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, doubl
 #pragma unroll
           for (int j = 0; j < V; ++j) mass += weight_bits(log2_weight(raw[a].get(j), m, c), shift);
         mass -= 4 * V * kUnitsBase;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
+        mass = wave_total(mass);
       }
       if (lane == 0) out.mass[p] = mass;
     }
@@ -387,10 +414,10 @@ __device__ __forceinline__ float row_max(const Pieces& p, int A, uint32_t* lds) 
   return group_max<NT>(bad ? __builtin_nanf("") : m, lds);
 }
 
-// masses (and counts, for top-k) of the classes of [begin, end), added into `mass` and `count` by NT threads
+// masses (and counts) of the classes of [begin, end), added into `mass` and `count` by NT threads
 template <typename T, int NT>
 __device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, int end, float m, const Row& r, int shift,
-                                            uint64_t* mass, uint32_t* count) {
+                                            uint64_t* mass, uint32_t* count, bool counts) {
   constexpr int V = Vec16<T>::n;
   for_each_vec<T, NT>(x, begin, end, threadIdx.x, [&](const float (&v)[V], int) {
     uint64_t u[V];
@@ -405,7 +432,7 @@ __device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, 
       if (y[j] >= kFloorLog2) {
         const int b = weight_bin(y[j]);
         atomicAdd((unsigned long long*)&mass[b], (unsigned long long)u[j]);
-        if (r.k > 0) atomicAdd(&count[b], 1u);
+        if (counts) atomicAdd(&count[b], 1u);
       }
     }
   });
@@ -473,16 +500,8 @@ __device__ __forceinline__ void scan_classes(RowWork<NT>& w, bool by_mass, uint6
       cs += c[j];
       ss += s[j];
     }
-    uint32_t ci = cs;
-    uint64_t si = ss;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t co = __shfl_up(ci, off, 64);
-      const uint64_t so = __shfl_up(si, off, 64);
-      if (l >= off) { ci += co; si += so; }
-    }
-    uint32_t ca = ci - cs;   // above this lane's classes
-    uint64_t sa = si - ss;
+    uint32_t ca = wave_scan(cs) - cs;   // above this lane's classes
+    uint64_t sa = wave_scan(ss) - ss;
     int bin = -1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -523,34 +542,51 @@ __device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<NT>& w
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
   if (threadIdx.x == 0) { w.listed = true; w.lo = 0xffffffffu; w.hi = 0; }
-  // A little more than the class' range: one comparison for a load's values together where they are all below it, else two
-  // for each.  A wave appends what it finds to a list of its own; whether it is of the class is seen afterwards, on
-  // the list (float64 in this loop would run for every second load of a wave).
-  const double step = 1.0 / kPerHalving / v.r.c, slack = 1e-6 * (fabs((double)v.m) + (bin + 1) * step) + 1e-37;
-  const float top = (float)((double)v.m - bin * step + slack);
-  const float bottom = bin == kLastBin ? -3.4028235e38f : (float)((double)v.m - (bin + 1) * step - slack);
-  const uint32_t inv = (65536u + (v.seg_len >> 11) - 1) / (v.seg_len >> 11);   // segments are multiples of 2,048
-  uint32_t n = 0;   // the same in every lane
-  for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int i) {
-    float most = g[0];
-#pragma unroll
-    for (int j = 1; j < V; ++j) most = fmaxf(most, g[j]);
-    if (!__any(most >= bottom)) return;
-    const uint32_t seg = ((uint32_t)(i >> 11) * inv) >> 16;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const bool hit = g[j] <= top && g[j] >= bottom;
-      const uint64_t mask = __ballot(hit);
-      if (mask) {
-        const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-        if (hit && at < kList) {
-          w.list[wave][at] = __float_as_uint(g[j]);
-          w.list_seg[wave][at] = (uint8_t)seg;
+  uint32_t n = 0;   // of this wave's list, the same in every lane
+  if (v.values) {
+    // the class lies in one stretch of each segment's values: lane s has the stretch of segment s
+    const int bin0 = lane * kBins + bin;
+    const uint32_t from = lane < v.n_seg ? v.seg_first[bin0] : 0, to = lane < v.n_seg ? v.seg_first[bin0 + 1] : 0;
+    for (int s = wave; s < v.n_seg; s += NT / 64) {
+      const uint32_t first = __shfl(from, s, 64), last = __shfl(to, s, 64);
+      for (uint32_t i = first + lane; i < last; i += 64) {
+        const uint32_t at = n + (i - first);
+        if (at < kList) {
+          w.list[wave][at] = __float_as_uint(v.values[s * v.seg_len + i]);
+          w.list_seg[wave][at] = (uint8_t)s;
         }
-        n += (uint32_t)__popcll(mask);
       }
+      n += last - first;
     }
-  });
+  } else {
+    // A little more than the class' range: one comparison for a load's values together where they are all below it, else two
+    // for each.  A wave appends what it finds to a list of its own; whether it is of the class is seen afterwards, on
+    // the list (float64 in this loop would run for every second load of a wave).
+    const double step = 1.0 / kPerHalving / v.r.c, slack = 1e-6 * (fabs((double)v.m) + (bin + 1) * step) + 1e-37;
+    const float top = (float)((double)v.m - bin * step + slack);
+    const float bottom = bin == kLastBin ? -3.4028235e38f : (float)((double)v.m - (bin + 1) * step - slack);
+    const uint32_t inv = (65536u + (v.seg_len >> 11) - 1) / (v.seg_len >> 11);   // segments are multiples of 2,048
+    for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int i) {
+      float most = g[0];
+#pragma unroll
+      for (int j = 1; j < V; ++j) most = fmaxf(most, g[j]);
+      if (!__any(most >= bottom)) return;
+      const uint32_t seg = ((uint32_t)(i >> 11) * inv) >> 16;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const bool hit = g[j] <= top && g[j] >= bottom;
+        const uint64_t mask = __ballot(hit);
+        if (mask) {
+          const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+          if (hit && at < kList) {
+            w.list[wave][at] = __float_as_uint(g[j]);
+            w.list_seg[wave][at] = (uint8_t)seg;
+          }
+          n += (uint32_t)__popcll(mask);
+        }
+      }
+    });
+  }
   __syncthreads();
   if (lane == 0) {
     w.list_n[wave] = n < kList ? n : kList;
@@ -676,8 +712,7 @@ __device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<NT>& w
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (64 * j + lane < bin) mass += v.seg_hist[s * kBins + 64 * j + lane];
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) mass += __shfl_xor(mass, off, 64);
+      mass = wave_total(mass);
       if (lane == 0) {
         w.seg_mass[s] = mass;
         w.seg_ties[s] = 0;
@@ -706,11 +741,8 @@ __device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<NT>& w
           ties += g[j] == cut.value;
         }
       });
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) {
-        mass += __shfl_xor(mass, off, 64);
-        ties += __shfl_xor(ties, off, 64);
-      }
+      mass = wave_total(mass);
+      ties = wave_total(ties);
       if (lane == 0) {
         w.seg_mass[s] = mass;
         w.seg_ties[s] = ties;
@@ -746,12 +778,7 @@ __device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, c
       uint32_t tie = 0;
 #pragma unroll
       for (int j = 0; j < V; ++j) tie += g[j] == cut.value;
-      uint32_t run = tie;
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const uint32_t o = __shfl_up(run, off, 64);
-        if (lane >= off) run += o;
-      }
+      const uint32_t run = wave_scan(tie);
       tie_before = run - tie;
       if constexpr (NT > 64) {
         __syncthreads();
@@ -763,7 +790,7 @@ __device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, c
           tie_all += w.red32[o];
         }
       } else {
-        tie_all = __shfl(run, 63, 64);
+        tie_all = last_lane(run);
       }
     }
     uint64_t sum = 0;
@@ -777,12 +804,7 @@ __device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, c
       }
       sum += u[j];
     }
-    uint64_t run = sum;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint64_t o = __shfl_up(run, off, 64);
-      if (lane >= off) run += o;
-    }
+    const uint64_t run = wave_scan(sum);
     uint64_t before = run - sum, here = 0;
     if constexpr (NT > 64) {
       __syncthreads();
@@ -794,7 +816,7 @@ __device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, c
         here += w.red64[o];
       }
     } else {
-      here = __shfl(run, 63, 64);
+      here = last_lane(run);
     }
     if (here > target) {   // it is in this tile, and one thread has it
       if (before <= target && before + sum > target) {
@@ -832,22 +854,11 @@ __device__ __forceinline__ void draw_filtered(const RowView<T>& v, RowWork<NT>& 
     const int lane = threadIdx.x;
     const uint32_t keep = one ? cut.ties : 0;
     const uint32_t ties = lane < v.n_seg ? w.seg_ties[lane] : 0;
-    uint32_t tie_run = ties;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint32_t o = __shfl_up(tie_run, off, 64);
-      if (lane >= off) tie_run += o;
-    }
-    const uint32_t tie_before = tie_run - ties;
+    const uint32_t tie_before = wave_scan(ties) - ties;
     const uint32_t left = tie_before < keep ? keep - tie_before : 0;
     const uint64_t mass = (lane < v.n_seg ? w.seg_mass[lane] : 0) + (uint64_t)(ties < left ? ties : left) * one;
-    uint64_t run = mass;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const uint64_t o = __shfl_up(run, off, 64);
-      if (lane >= off) run += o;
-    }
-    const uint64_t target = draw_target(q.uniforms[row], __shfl(run, 63, 64));
+    const uint64_t run = wave_scan(mass);
+    const uint64_t target = draw_target(q.uniforms[row], last_lane(run));
     if (run > target && run - mass <= target) {   // one lane
       w.found = lane;
       w.found_target = target - (run - mass);
@@ -874,12 +885,7 @@ __device__ __forceinline__ void draw_pieces(const RowView<T>& v, RowWork<NT>& w,
   // the piece's mass relative to the row's maximum: exact where that is the piece's own, rounded to 53 bits elsewhere
   const double y = ref > -INFINITY ? log2_weight(ref, v.m, v.r.c) : -1e9;
   const uint64_t mass = y == 0.0 ? raw : y >= kFloorLog2 ? (uint64_t)rint((double)raw * exp2(y)) : 0;
-  uint64_t run = mass;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint64_t o = __shfl_up(run, off, 64);
-    if (lane >= off) run += o;
-  }
+  const uint64_t run = wave_scan(mass);
   uint64_t before = run - mass, total = 0;
   if constexpr (NT > 64) {
     __syncthreads();
@@ -891,7 +897,7 @@ __device__ __forceinline__ void draw_pieces(const RowView<T>& v, RowWork<NT>& w,
       total += w.red64[o];
     }
   } else {
-    total = __shfl(run, 63, 64);
+    total = last_lane(run);
   }
   const uint64_t target = draw_target(q.uniforms[row], total);
   if (before <= target && before + mass > target) {   // one thread
@@ -970,6 +976,8 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const T* __restrict__ l
   v.seg_len = kWaveRow;
   v.seg_hist = hist;
   v.seg_count = count;
+  v.seg_first = nullptr;
+  v.values = nullptr;
   const Pieces p{piece_mass, piece_max};
   const bool hists = filtered(v.r);
   sum_pieces(v.x, A, v.r.c, v.shift, 0, (A + piece_length<T>() - 1) / piece_length<T>(), 0, 1, p, !hists && !v.r.greedy);
@@ -978,7 +986,7 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const T* __restrict__ l
   if (hists && v.m > -INFINITY) {
     for (int i = threadIdx.x; i < kBins; i += 64) { hist[i] = 0; count[i] = 0; }
     __syncthreads();
-    add_classes<T, 64>(v.x, 0, A, v.m, v.r, v.shift, hist, count);
+    add_classes<T, 64>(v.x, 0, A, v.m, v.r, v.shift, hist, count, v.r.k > 0);
     __syncthreads();
   }
   draw_row(v, w, q, row, p);
@@ -986,26 +994,30 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const T* __restrict__ l
 
 // Longer rows: how a batch is cut.  What a row leaves in the workspace: its pieces' masses and maxima and, where it has
 // filters, its segments' classes.
+constexpr int64_t kFewElements = (int64_t)8 << 20;
 struct SamplePlan {
+  int64_t bytes;
   int n_seg, seg_len, n_piece;
   int64_t group;                         // rows that go through the three launches together
   uint64_t* piece_mass;                  // [B][n_piece]
   uint64_t* seg_hist;                    // [group][n_seg][kBins]
   uint32_t* seg_count;                   // [group][n_seg][kBins]
   float* piece_max;                      // [B][n_piece]
+  uint32_t* seg_first;                   // [B][n_seg][kBins], and
+  float* values;                         // [B][n_seg][seg_len]: the values by class, where the rows are few; else NULL
 };
 
 constexpr int kPartThreads = 256;
 
-// a workgroup per segment: the pieces' maxima, and their masses where that is all a row needs
+// a workgroup for `per` pieces: their maxima, and their masses where that is all a row needs
 template <typename T>
 __global__ __launch_bounds__(kPartThreads) void sample_pieces_kernel(const T* __restrict__ logits, int64_t stride, int A,
-                                                                     SampleArgs q, SamplePlan plan, int64_t row0) {
-  const int64_t row = row0 + blockIdx.x / plan.n_seg;
-  const int seg = blockIdx.x % plan.n_seg;
+                                                                     SampleArgs q, SamplePlan plan, int64_t row0, int per) {
+  const int n = (A + piece_length<T>() - 1) / piece_length<T>();
+  const uint32_t groups = (n + per - 1) / per;
+  const int64_t row = row0 + blockIdx.x / groups;
   const Row r = row_settings(q, row);
-  const int per = plan.seg_len / piece_length<T>(), n = (A + piece_length<T>() - 1) / piece_length<T>();
-  const int first = seg * per, last = first + per < n ? first + per : n;
+  const int first = (int)(blockIdx.x % groups) * per, last = first + per < n ? first + per : n;
   const Pieces p{plan.piece_mass + row * plan.n_piece, plan.piece_max + row * plan.n_piece};
   sum_pieces(logits + row * stride, A, r.c, q.shift, first, last, threadIdx.x >> 6, kPartThreads / 64, p,
              !r.greedy && !filtered(r));
@@ -1025,15 +1037,38 @@ __global__ __launch_bounds__(kPartThreads) void sample_classes_kernel(const T* _
   const float m = row_max<T, kPartThreads>(p, A, red);
   if (!(m > -INFINITY)) return;
   static_assert(kPartThreads == kBins, "a thread for each class");
-  hist[threadIdx.x] = 0;
-  count[threadIdx.x] = 0;
+  const int b = threadIdx.x;
+  hist[b] = 0;
+  count[b] = 0;
   __syncthreads();
+  const bool counts = r.k > 0 || plan.values;
   const int begin = seg * plan.seg_len, end = begin + plan.seg_len < A ? begin + plan.seg_len : A;
-  add_classes<T, kPartThreads>(logits + row * stride, begin, end, m, r, q.shift, hist, count);
+  const T* x = logits + row * stride;
+  add_classes<T, kPartThreads>(x, begin, end, m, r, q.shift, hist, count, counts);
   __syncthreads();
-  const int64_t at = ((row - row0) * plan.n_seg + seg) * kBins + threadIdx.x;
-  plan.seg_hist[at] = hist[threadIdx.x];
-  if (r.k > 0) plan.seg_count[at] = count[threadIdx.x];
+  const int64_t part = (row - row0) * plan.n_seg + seg;
+  const uint32_t n = count[b];
+  plan.seg_hist[part * kBins + b] = hist[b];
+  if (counts) plan.seg_count[part * kBins + b] = n;
+  if (!plan.values) return;
+  // A few rows leave no work for most of the card while a workgroup each looks for the values of a class in them: here they are
+  // put in the order of their classes, by all the segments' workgroups.
+  const int lane = b & 63, wave = b >> 6;
+  uint32_t run = wave_scan(n);
+  if (lane == 63) red[wave] = run;
+  __syncthreads();   // every count has been read
+  for (int w = 0; w < wave; ++w) run += red[w];
+  plan.seg_first[part * kBins + b] = run - n;
+  count[b] = run - n;
+  __syncthreads();
+  float* values = plan.values + part * plan.seg_len;
+  for_each_vec<T, kPartThreads>(x, begin, end, b, [&](const float (&g)[Vec16<T>::n], int) {
+#pragma unroll
+    for (int j = 0; j < Vec16<T>::n; ++j) {
+      const double y = log2_weight(g[j], m, r.c);
+      if (y >= kFloorLog2) values[atomicAdd(&count[weight_bin(y)], 1u)] = g[j];
+    }
+  });
 }
 
 // a workgroup per row: the rest
@@ -1051,6 +1086,8 @@ __global__ __launch_bounds__(NT) void sample_finish_kernel(const T* __restrict__
   v.seg_len = plan.seg_len;
   v.seg_hist = plan.seg_hist + blockIdx.x * (int64_t)plan.n_seg * kBins;
   v.seg_count = plan.seg_count + blockIdx.x * (int64_t)plan.n_seg * kBins;
+  v.seg_first = plan.values ? plan.seg_first + blockIdx.x * (int64_t)plan.n_seg * kBins : nullptr;
+  v.values = plan.values ? plan.values + blockIdx.x * (int64_t)plan.n_seg * plan.seg_len : nullptr;
   const Pieces p{plan.piece_mass + row * plan.n_piece, plan.piece_max + row * plan.n_piece};
   v.m = row_max<T, NT>(p, A, w.red32);
   draw_row(v, w, q, row, p);
@@ -1070,12 +1107,13 @@ static SamplePlan sample_plan(int64_t B, int64_t A, void* workspace) {
   if (p.group > B) p.group = B;
   // segments of about 8,192 actions (the last pass scans one of them), of fewer where the rows are few
   int64_t n = (A + 8191) / 8192;
-  const int64_t few = 2048 / p.group, most = A / 4096;
-  if (n < few && n < most) n = few < most ? few : most;
+  const int64_t few = 2048 / p.group, most = (A + 4095) / 4096;
+  if (n < few) n = few < most ? few : most;
   if (n > kMaxParts) n = kMaxParts;
   p.seg_len = (int)(((A + n - 1) / n + 2047) / 2048 * 2048);
   p.n_seg = (int)((A + p.seg_len - 1) / p.seg_len);
   p.n_piece = (int)((A + kPiece - 1) / kPiece);
+  const bool by_class = B * A <= kFewElements;
   char* at = (char*)workspace;
   p.piece_mass = (uint64_t*)at;
   at += B * p.n_piece * 8;
@@ -1083,14 +1121,19 @@ static SamplePlan sample_plan(int64_t B, int64_t A, void* workspace) {
   at += p.group * p.n_seg * kBins * 8;
   p.seg_count = (uint32_t*)at;
   at += p.group * p.n_seg * kBins * 4;
+  p.seg_first = (uint32_t*)at;
+  if (by_class) at += p.group * p.n_seg * kBins * 4;
+  p.values = by_class ? (float*)at : nullptr;
+  if (by_class) at += p.group * p.n_seg * p.seg_len * 4;
   p.piece_max = (float*)at;
+  at += B * p.n_piece * 4;
+  p.bytes = at - (char*)workspace;
   return p;
 }
 
 static size_t sample_workspace(int64_t B, int64_t A) {
   if (B <= 0 || A <= kWaveRow) return 0;
-  const SamplePlan p = sample_plan(B, A, nullptr);
-  return (size_t)B * p.n_piece * 12 + (size_t)p.group * p.n_seg * kBins * 12;
+  return (size_t)sample_plan(B, A, nullptr).bytes;
 }
 
 template <typename T>
@@ -1116,15 +1159,17 @@ static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, con
   const int64_t group = filters ? p.group : B;
   for (int64_t row0 = 0; row0 < B; row0 += group) {
     const int64_t rows = row0 + group < B ? group : B - row0;
-    const int parts = (int)(rows * p.n_seg);
-    sample_pieces_kernel<T><<<parts, kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    // a piece for each wave, or two where that makes more than enough workgroups
+    const int pieces = (int)((A + piece_length<T>() - 1) / piece_length<T>());
+    const int per = rows * pieces >= 65536 ? 8 : 4;
+    sample_pieces_kernel<T><<<(int)(rows * ((pieces + per - 1) / per)), kPartThreads, 0, s>>>(logits, stride, (int)A, q, p,
+                                                                                            row0, per);
     if (int rc = check_launch()) return rc;
     if (filters) {
-      sample_classes_kernel<T><<<parts, kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
+      sample_classes_kernel<T><<<(int)(rows * p.n_seg), kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
       if (int rc = check_launch()) return rc;
     }
     // a thread for each piece of a row; else smaller workgroups, more rows side by side, where the rows are many
-    const int pieces = (int)((A + piece_length<T>() - 1) / piece_length<T>());
     if (pieces > 512)
       sample_finish_kernel<T, 1024><<<(int)rows, 1024, 0, s>>>(logits, stride, (int)A, q, p, row0);
     else if (rows < 512 || pieces > 256)
@@ -1151,8 +1196,8 @@ PARLHIP_EXPORT int parlhip_logits_sample(const void* logits, int dtype, int64_t 
                                          void* workspace, size_t workspace_bytes, parlhip_stream_t stream) {
   if (B < 0 || A < 1 || row_stride < A) return PARLHIP_EINVAL;
   if (dtype != PARLHIP_F32 && dtype != PARLHIP_BF16 && dtype != PARLHIP_F16) return PARLHIP_ENOSUP;
-  // one launch's threads: 64 for a row at most, or 256 for each of its segments
-  if (A > kSampleMaxActions || B > 0xffffffffLL / (A <= kWaveRow ? 64 : 256 * kMaxParts)) return PARLHIP_ENOSUP;
+  // one launch's threads: 64 for a row at most, or 256 for every eight of its 1,024 pieces
+  if (A > kSampleMaxActions || B > 0xffffffffLL / (A <= kWaveRow ? 64 : 256 * 128)) return PARLHIP_ENOSUP;
   if (!temperature && !(temperature_all >= 0.f && temperature_all < INFINITY)) return PARLHIP_EINVAL;
   if (!top_p && !(top_p_all >= 0.f)) return PARLHIP_EINVAL;
   if (!min_p && !(min_p_all >= 0.f && min_p_all <= 1.f)) return PARLHIP_EINVAL;
