@@ -5,7 +5,14 @@ What runs where: the model forward / backward, Normal / Categorical log-probabil
 surrogate and Adam are PyTorch-ROCm; the per-minibatch advantage normalisation
 `(adv - adv.mean()) / (adv.std() + 1e-8)` (ppo.py:124-127, unbiased std) is the HIP kernel
 `parlhip_adv_normalize_f32` (advantages carry no gradient).  The GAE scan and the minibatch
-gather that feed learn() live in parl_amd.storage.RolloutStorage."""
+gather that feed learn() live in parl_amd.storage.RolloutStorage.
+
+`fused_policy=True` (discrete actions on the device) is for action sets the size of a vocabulary: log-probabilities,
+entropies and their gradient (`ops.logits_log_prob`), the draw (`ops.logits_sample`, with uniforms of torch's generator) and
+the clipping of the global gradient norm (`ops.clip_grad_norm_`) are the library's kernels instead of torch's
+Categorical and clip_grad_norm_, which materialise several arrays of the logits' size.  The policy may return float32,
+bfloat16 or float16 logits, and an action of -1 marks a row that is no decision: log-probability and entropy 0,
+no gradient from either."""
 import torch
 import torch.nn as nn
 from torch.distributions import Categorical, Normal
@@ -27,7 +34,8 @@ class PPO(Algorithm):
                  max_grad_norm=0.5,
                  use_clipped_value_loss=True,
                  norm_adv=True,
-                 continuous_action=False):
+                 continuous_action=False,
+                 fused_policy=False):
         for m in ('value', 'policy'):  # check_model_method, parl/utils/utils.py:217-243
             assert callable(getattr(model, m, None)), '%s: model needs a `%s` method' % (self.__class__.__name__, m)
         # the argument checks of ppo.py:57-65
@@ -40,6 +48,8 @@ class PPO(Algorithm):
         assert isinstance(use_clipped_value_loss, bool)
         assert isinstance(norm_adv, bool)
         assert isinstance(continuous_action, bool)
+        assert isinstance(fused_policy, bool)
+        assert not (fused_policy and continuous_action), 'fused_policy: discrete actions only'
         super(PPO, self).__init__(model)
         self.clip_param = clip_param
         self.value_loss_coef = value_loss_coef
@@ -48,6 +58,7 @@ class PPO(Algorithm):
         self.use_clipped_value_loss = use_clipped_value_loss
         self.norm_adv = norm_adv
         self.continuous_action = continuous_action
+        self.fused_policy = fused_policy
         if torch.cuda.is_available():  # ppo.py:75-76
             self.model = model.to(torch.device('cuda'))
         self.optimizer = torch.optim.Adam(self.model.parameters(), lr=initial_lr, eps=eps)
@@ -61,8 +72,11 @@ class PPO(Algorithm):
 
     def _losses(self, obs, action, old_value, ret, old_logp, adv):
         """the three terms of the PPO objective for one minibatch (ppo.py:104-148)"""
-        dist = self._dist(obs)
-        logp, entropy = dist.log_prob(action), dist.entropy()
+        if self.fused_policy:
+            logp, entropy = ops.logits_log_prob(self.model.policy(obs), action.to(torch.int64))
+        else:
+            dist = self._dist(obs)
+            logp, entropy = dist.log_prob(action), dist.entropy()
         if self.continuous_action:  # independent Normal per action dimension
             logp, entropy = logp.sum(1), entropy.sum(1)
         if self.norm_adv:  # ppo.py:124-127 on the device kernel (unbiased std, + 1e-8); no gradient
@@ -91,7 +105,8 @@ class PPO(Algorithm):
         loss.backward()
         if self.grad_hook is not None:
             self.grad_hook(self.model)
-        nn.utils.clip_grad_norm_(self.model.parameters(), self.max_grad_norm)
+        clip_grad_norm_ = ops.clip_grad_norm_ if self.fused_policy else nn.utils.clip_grad_norm_
+        clip_grad_norm_(self.model.parameters(), self.max_grad_norm)
         self.optimizer.step()
         return value_loss.item(), action_loss.item(), entropy_loss.item()
 
@@ -99,6 +114,12 @@ class PPO(Algorithm):
     def sample(self, obs):
         """ppo.py:160-187: (value, action, action_log_probs, action_entropy)"""
         value = self.model.value(obs)
+        if self.fused_policy:
+            logits = self.model.policy(obs)
+            uniforms = torch.rand(logits.shape[:-1], dtype=torch.float64, device=logits.device)
+            action, _ = ops.logits_sample(logits, uniforms)
+            log_probs, entropy = ops.logits_log_prob(logits, action)
+            return value, action, log_probs, entropy
         dist = self._dist(obs)
         action = dist.sample()
         if self.continuous_action:
@@ -111,6 +132,8 @@ class PPO(Algorithm):
         if self.continuous_action:
             action, _ = self.model.policy(obs)
             return action
+        if self.fused_policy:
+            return self.model.policy(obs).argmax(dim=-1, keepdim=True)
         return Categorical(logits=self.model.policy(obs)).probs.argmax(dim=-1, keepdim=True)
 
     @torch.no_grad()

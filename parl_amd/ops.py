@@ -946,7 +946,7 @@ def grad_norm(tensors):
     return N.torch_ops().grad_norm(tensors)
 
 
-def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False, out=None):
+def clip_grad_norm_(parameters, max_norm, *, error_if_nonfinite=False, out=None):
     """torch.nn.utils.clip_grad_norm_(parameters, max_norm) (parl/algorithms/torch/a2c.py:76-78) over any number of
     parameters whose gradients are float32 / bfloat16 / float16 (mixed): every .grad times min(1, max_norm / (norm + 1e-6)),
     in two launches for up to 168 gradients.  Returns the norm before clipping, a float32 scalar tensor on the device (no
