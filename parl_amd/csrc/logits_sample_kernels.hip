@@ -21,7 +21,7 @@
 //               values in LDS, by the same histogram over ever fewer bits (or on the row itself, where a flat row puts
 //               more values into one class than the list takes).  The classes above the border and the list give the
 //               kept mass of every segment, and the segment that the draw falls into is scanned.
-// Rows of up to 2,048 actions do that in one wave each.  Above, every pass over the rows is a launch of its own over segments of
+// Rows of up to 4,096 actions do that in one wave each.  Above, every pass over the rows is a launch of its own over segments of
 // all rows, which fills the card whether the rows are many or few and long, and a workgroup per row finishes.
 #include "common.hpp"
 #include "logits_common.hpp"
@@ -196,18 +196,29 @@ __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__
 #pragma unroll
   for (int off = LP / 2; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
   bool keep = u > 0;
-  if (__any(r.k > 0 || r.top_p < 1.f)) {
+  if (__any(r.k == 1)) {   // the first of the largest
+    const uint64_t largest = __ballot(x == m) >> (threadIdx.x % 64 / LP * LP);
+    if (r.k == 1) keep = keep && x == m && !(largest & (((uint64_t)1 << sub) - 1));
+  }
+  if (__any(r.k > 1 || r.top_p < 1.f)) {
     int position = 0;
     uint64_t before = 0;
-    for (int j = 0; j < LP; ++j) {
-      const float xj = __shfl(x, j, LP);
-      const uint64_t uj = __shfl(u, j, LP);
-      if (uj > 0 && (xj > x || (xj == x && j < sub))) {
-        ++position;
-        before += uj;
+    for (int j = 0; j < A; ++j) {
+      float xj;
+      uint64_t uj;
+      if constexpr (LP == 64) {   // one row: through scalar registers
+        xj = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(x), j));
+        uj = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, j) |
+             (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), j) << 32;
+      } else {
+        xj = __shfl(x, j, LP);
+        uj = __shfl(u, j, LP);
       }
+      const bool above = xj > x || (xj == x && j < sub);   // one without weight adds none, and is above none that has
+      position += above;
+      before += above ? uj : 0;
     }
-    keep = keep && (r.k == 0 || position < r.k);
+    keep = keep && (r.k <= 1 || position < r.k);
     uint64_t mass_k = keep ? u : 0;
 #pragma unroll
     for (int off = LP / 2; off > 0; off >>= 1) mass_k += __shfl_xor(mass_k, off, 64);
@@ -362,6 +373,7 @@ __device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, doubl
   const int lane = threadIdx.x & 63;
   for (int p = first + wave; p < last; p += waves) {
     const int base = p * kLen + lane * V;
+    const int loads = A - p * kLen >= kLen ? 4 : (A - p * kLen + 64 * V - 1) / (64 * V);   // of the wave
     Vec16<T> raw[4];
     if (p * kLen + kLen <= A) {
 #pragma unroll
@@ -369,13 +381,15 @@ __device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, doubl
     } else {
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
-        float g[V];
+        const int i0 = base + a * 64 * V;
+        if (i0 + V <= A) {
+          raw[a].load(x + i0);
+        } else {
+          float g[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int i = base + a * 64 * V + j;
-          g[j] = i < A ? to_f32(x[i]) : -INFINITY;
+          for (int j = 0; j < V; ++j) g[j] = i0 + j < A ? to_f32(x[i0 + j]) : -INFINITY;
+          raw[a].pack(g);   // exact: they came from this type
         }
-        raw[a].pack(g);   // exact: they came from this type
       }
     }
     float m = -INFINITY;   // a NaN stays
@@ -388,10 +402,12 @@ __device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, doubl
       uint64_t mass = 0;
       if (m > -INFINITY) {
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < 4; ++a) {
+          if (a >= loads) break;
 #pragma unroll
           for (int j = 0; j < V; ++j) mass += weight_bits(log2_weight(raw[a].get(j), m, c), shift);
-        mass -= 4 * V * kUnitsBase;
+        }
+        mass -= (uint64_t)(loads * V) * kUnitsBase;
         mass = wave_total(mass);
       }
       if (lane == 0) out.mass[p] = mass;
@@ -535,6 +551,13 @@ __device__ __forceinline__ void for_listed(RowWork<NT>& w, F&& f) {
   for (uint32_t i = threadIdx.x & 63; i < n; i += 64) f(w.list[wave][i], (int)w.list_seg[wave][i]);
 }
 
+// f(value) for class `bin` of segment s, where the values lie by class; by the lanes of a wave
+template <typename T, typename F>
+__device__ __forceinline__ void for_stretch(const RowView<T>& v, int s, int bin, F&& f) {
+  const uint32_t last = v.seg_first[s * kBins + bin + 1];
+  for (uint32_t i = v.seg_first[s * kBins + bin] + (threadIdx.x & 63); i < last; i += 64) f(v.values[s * v.seg_len + i]);
+}
+
 // The values of class `bin` -> w.list (w.listed: all of them), their range -> w.lo, w.hi.
 template <typename T, int NT>
 __device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<NT>& w, int bin) {
@@ -604,6 +627,8 @@ __device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<NT>& w
   };
   if (w.listed)
     for (uint32_t i = lane; i < n; i += 64) w.list[wave][i] = of_class(__uint_as_float(w.list[wave][i]));
+  else if (v.values)
+    for (int s = wave; s < v.n_seg; s += NT / 64) for_stretch(v, s, bin, of_class);
   else
     for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int) {
 #pragma unroll
@@ -618,8 +643,8 @@ __device__ __forceinline__ void gather_class(const RowView<T>& v, RowWork<NT>& w
 
 // The value at which the count (or mass) counted from the top reaches `need`, inside the listed class.
 template <typename T, int NT>
-__device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<NT>& w, uint64_t above_mass, uint64_t above_count,
-                                      bool by_mass, uint64_t need) {
+__device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<NT>& w, int bin, uint64_t above_mass,
+                                      uint64_t above_count, bool by_mass, uint64_t need) {
   constexpr int V = Vec16<T>::n;
   uint32_t lo = w.lo, hi = w.hi;
   const bool listed = w.listed;
@@ -639,6 +664,8 @@ __device__ __forceinline__ Cut refine(const RowView<T>& v, RowWork<NT>& w, uint6
     };
     if (listed)
       for_listed(w, [&](uint32_t k, int) { add(k); });
+    else if (v.values)
+      for (int s = threadIdx.x >> 6; s < v.n_seg; s += NT / 64) for_stretch(v, s, bin, [&](float x) { add(value_key(x)); });
     else
       for_each_vec<T, NT>(v.x, 0, v.A, threadIdx.x, [&](const float (&g)[V], int) {
 #pragma unroll
@@ -677,7 +704,7 @@ __device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<NT>& w, uin
       for (int j = 0; j < kKeep; ++j) keep[j] = w.mass[(threadIdx.x + j * NT) % kBins];
       gather_class(v, w, bin);
       listed = bin;
-      cut = refine(v, w, am, ac, false, (uint64_t)v.r.k);
+      cut = refine(v, w, bin, am, ac, false, (uint64_t)v.r.k);
       mass_k = cut.above + (uint64_t)cut.ties * weight_units(log2_weight(cut.value, v.m, v.r.c), v.shift);
       __syncthreads();
 #pragma unroll
@@ -691,7 +718,7 @@ __device__ __forceinline__ Cut find_cut(const RowView<T>& v, RowWork<NT>& w, uin
     const uint64_t am = w.above_mass;
     if (bin != listed) gather_class(v, w, bin);
     listed = bin;
-    const Cut p = refine(v, w, am, 0, true, need);
+    const Cut p = refine(v, w, bin, am, 0, true, need);
     if (p.value > cut.value || (p.value == cut.value && p.ties < cut.ties)) cut = p;
   }
   return cut;
@@ -706,27 +733,37 @@ __device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<NT>& w
   const int bin = weight_bin(fmax(y_cut, v.r.ymin));   // above it everything is kept, below it nothing
   if (bin != listed) gather_class(v, w, bin);
   __syncthreads();
-  if (w.listed) {
+  if (w.listed || v.values) {
     for (int s = wave; s < v.n_seg; s += kWaves) {
       uint64_t mass = 0;
+      uint32_t ties = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (64 * j + lane < bin) mass += v.seg_hist[s * kBins + 64 * j + lane];
+      if (!w.listed) {
+        for_stretch(v, s, bin, [&](float x) {
+          const double y = log2_weight(x, v.m, v.r.c);
+          ties += x == cut.value;
+          mass += x > cut.value && y >= v.r.ymin ? weight_units(y, v.shift) : 0;
+        });
+        ties = wave_total(ties);
+      }
       mass = wave_total(mass);
       if (lane == 0) {
         w.seg_mass[s] = mass;
-        w.seg_ties[s] = 0;
+        w.seg_ties[s] = ties;
       }
     }
     __syncthreads();
-    for_listed(w, [&](uint32_t k, int s) {
-      const float x = key_value(k);
-      const double y = log2_weight(x, v.m, v.r.c);
-      if (x == cut.value)   // x is NaN where there is none
-        atomicAdd(&w.seg_ties[s], 1u);
-      else if (x > cut.value && y >= v.r.ymin)
-        atomicAdd((unsigned long long*)&w.seg_mass[s], (unsigned long long)weight_units(y, v.shift));
-    });
+    if (w.listed)
+      for_listed(w, [&](uint32_t k, int s) {
+        const float x = key_value(k);
+        const double y = log2_weight(x, v.m, v.r.c);
+        if (x == cut.value)   // x is NaN where there is none
+          atomicAdd(&w.seg_ties[s], 1u);
+        else if (x > cut.value && y >= v.r.ymin)
+          atomicAdd((unsigned long long*)&w.seg_mass[s], (unsigned long long)weight_units(y, v.shift));
+      });
   } else {   // a flat row: over the whole of it again
     for (int s = wave; s < v.n_seg; s += kWaves) {
       const int begin = s * v.seg_len < v.A ? s * v.seg_len : v.A, end = begin + v.seg_len < v.A ? begin + v.seg_len : v.A;
@@ -957,7 +994,7 @@ __device__ __forceinline__ void draw_row(const RowView<T>& v, RowWork<NT>& w, co
 }
 
 // Rows of up to kWaveRow actions: one wave each.
-constexpr int kWaveRow = 2048;
+constexpr int kWaveRow = 4096;
 
 template <typename T>
 __global__ __launch_bounds__(64) void sample_wave_kernel(const T* __restrict__ logits, int64_t stride, int A, SampleArgs q) {
