@@ -23,6 +23,12 @@
 //               kept mass of every segment, and the segment that the draw falls into is scanned.
 // Rows of up to 4,096 actions do that in one wave each.  Above, every pass over the rows is a launch of its own over segments of
 // all rows, which fills the card whether the rows are many or few and long, and a workgroup per row finishes.
+//
+// Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 101 us, 55 us of which the 268 MB
+// would take; the pass is bound by the vector unit, which issues in 89 % of its slots, 25 instructions a value.  1,024 x 100,003
+// with top-p 0.95: 31 us for the maxima (HBM), 103 for the classes (28 instructions a value), 92 for the finish
+// (a pass over the row by each workgroup, and the chain of scans behind it).  One row of 131,072 with top-k and
+// top-p: 25 us, three launches and the finish's chain of 13 us.
 #include "common.hpp"
 #include "logits_common.hpp"
 
@@ -151,7 +157,7 @@ __device__ __forceinline__ uint64_t weight_units(double y, int shift) { return w
 // the class of a weight: six for each halving, 0 for the largest, 252 for 2^-42
 __device__ __forceinline__ int weight_bin(double y) { return (int)(y * -kPerHalving); }
 
-// u * mass rounded down to whole units; u is a multiple of 2^-53, so this is exact: the draw is the first action whose
+// u * mass rounded down to whole units, exactly (u itself is taken to a multiple of 2^-53): the draw is the first action whose
 // running mass exceeds it, and there always is one
 __device__ __forceinline__ uint64_t draw_target(double u, uint64_t mass) {
   u = u > 0.0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
@@ -173,7 +179,7 @@ __device__ __forceinline__ float log_prob_of(float x, float m, const Row& r, uin
 
 // ------------------------------------------------------------------------------------------------------------------
 // A <= 64: LP lanes share a row, a lane holds one action.  The position and the mass before an action are summed over
-// the row's lanes directly.
+// the row's lanes directly.  1,024 rows of 18 take 4 us (one launch), 65,536 of them 20 us, with top-p 39.
 template <typename T, int LP>
 __global__ __launch_bounds__(256) void sample_small_kernel(const T* __restrict__ logits, int64_t stride, int64_t B, int A,
                                                            SampleArgs q) {
