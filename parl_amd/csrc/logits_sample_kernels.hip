@@ -301,7 +301,7 @@ struct Pieces {          // of one row
 template <int NT>
 struct RowWork {
   static constexpr int kWaves = NT / 64;
-  static constexpr int kList = NT == 1024 ? 512 : 1024;   // of each wave
+  static constexpr int kList = NT == 1024 || NT == 64 ? 512 : 1024;   // of each wave
   uint64_t mass[kBins];                  // of the row, or of the class that is being taken apart
   uint32_t count[kBins];
   uint32_t list[kWaves][kList];          // the values (keys; 0: none) of a class and the segments that they are in

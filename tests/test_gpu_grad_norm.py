@@ -88,6 +88,21 @@ def test_clip_into_other_tensors(src, dst, ratio, dev):
     assert float(out_flat[0]) == 7 and float(out_flat[-1]) == 7       # the neighbours are as they were
 
 
+def test_a_tensor_of_more_than_32_bits_of_elements(dev):
+    from parl_amd import ops
+    n = 2**31 + 19
+    g = torch.full((n, ), 0.5, dtype=torch.bfloat16, device=dev)
+    g[-1] = 2.0
+    norm = ops.clip_grad_norm_(_params([g]), 0.25 * math.sqrt(n))
+    want = math.sqrt((n - 1) * 0.25 + 4.0)
+    assert float(norm) == pytest.approx(want, rel=2.0**-23)
+    c = 0.25 * math.sqrt(n) / (want + 1e-6)
+    for i in (0, 1, 2**30, 2**31 - 1, 2**31, n - 2):
+        assert float(g[i]) == pytest.approx(0.5 * c, rel=2.0**-8)
+    assert float(g[-1]) == pytest.approx(2.0 * c, rel=2.0**-8)
+    assert int((g[:-1] != g[0]).sum()) == 0
+
+
 def test_clip_of_other_layouts(dev):
     from parl_amd import ops
     g = torch.Generator(device=dev).manual_seed(1)

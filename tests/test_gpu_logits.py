@@ -103,6 +103,61 @@ def test_draw_of_long_rows_matches_float64(rows, A, dtype, settings, dev):
     check_draw(x, u, *ops.logits_sample(x, u, **settings), **settings)
 
 
+@pytest.mark.parametrize('rows,A,dtype', [(2, 1 << 20, torch.bfloat16), (2, 300000, torch.float32), (36, 250000, torch.bfloat16),
+                                          (3, 3500, torch.float32), (600, 17000, torch.bfloat16)])
+def test_draw_from_flat_rows(rows, A, dtype, dev):
+    """an untrained policy: many thousand values in the class that holds the border"""
+    from parl_amd import ops
+    x = _logits(rows, A, dtype, dev, 3, spread=0.3)
+    u = torch.rand(rows, generator=torch.Generator(device=dev).manual_seed(4), dtype=torch.float64, device=dev)
+    for s in (dict(top_p=0.6), dict(top_k=A // 3, top_p=0.99), dict(min_p=0.4)):
+        check_draw(x, u, *ops.logits_sample(x, u, **s), **s)
+
+
+@pytest.mark.parametrize('settings', [dict(), dict(top_k=20, top_p=0.8), dict(top_p=0.9, min_p=0.02), dict(temperature=0.0)])
+@pytest.mark.parametrize('A', [18, 300, 4097, 40000])
+def test_a_row_is_drawn_alike_in_any_batch(A, settings, dev):
+    """alone, in a few, in many (other kernels, other splits), with settings as numbers or for each row: the same bits"""
+    from parl_amd import ops
+    rows = 1200
+    x = _logits(rows, A, torch.bfloat16, dev, A)
+    u = torch.rand(rows, generator=torch.Generator(device=dev).manual_seed(4), dtype=torch.float64, device=dev)
+    a, lp = ops.logits_sample(x, u, **settings)
+    for part in (slice(0, 1), slice(5, 20), slice(100, 400)):
+        b, lq = ops.logits_sample(x[part], u[part], **settings)
+        assert torch.equal(a[part], b) and torch.equal(lp[part], lq)
+    each = {k: torch.full((rows, ), v, device=dev, dtype=torch.int32 if k == 'top_k' else torch.float32)
+            for k, v in settings.items()}
+    b, lq = ops.logits_sample(x, u, **each)
+    assert torch.equal(a, b) and torch.equal(lp, lq)
+
+
+def test_draw_from_more_rows_than_go_through_the_launches_together(dev):
+    from parl_amd import ops
+    rows, A = 66000, 4097
+    x = _logits(rows, A, torch.bfloat16, dev, 1)
+    u = torch.rand(rows, generator=torch.Generator(device=dev).manual_seed(4), dtype=torch.float64, device=dev)
+    for s in (dict(), dict(top_p=0.7)):
+        a, lp = ops.logits_sample(x, u, **s)
+        for part in (slice(0, 700), slice(65000, 66000)):
+            b, lq = ops.logits_sample(x[part], u[part], **s)
+            assert torch.equal(a[part], b) and torch.equal(lp[part], lq)
+    check_draw(x[-3:], u[-3:], a[-3:], lp[-3:], **s)
+
+
+@pytest.mark.parametrize('A', [20, 3000, 5000])
+def test_rows_whose_offsets_pass_32_bits(A, dev):
+    from parl_amd import ops
+    base = torch.empty(2**31 + 2 * A, dtype=torch.bfloat16, device=dev)
+    x = base.as_strided((3, A), (2**30, 1))
+    x.copy_(_logits(3, A, torch.bfloat16, dev, 8))
+    u = torch.rand(3, generator=torch.Generator(device=dev).manual_seed(4), dtype=torch.float64, device=dev)
+    for s in (dict(), dict(top_k=9, top_p=0.9)):
+        a, lp = ops.logits_sample(x, u, **s)
+        check_draw(x, u, a, lp, **s)
+    check_logp(x, a, 1.0, dev)
+
+
 @pytest.mark.parametrize('A', [18, 700, 5000, 70000])
 def test_draw_with_settings_for_each_row(A, dev):
     from parl_amd import ops
@@ -165,10 +220,11 @@ def test_draw_of_masked_and_bad_rows(A, dtype, settings, dev):
     assert torch.equal(b[:7], a[:7]) and torch.equal(b[11:], a[11:])
 
 
-def test_draw_at_the_ends_of_the_uniforms(dev):
+@pytest.mark.parametrize('A', [50, 3000, 9000])
+def test_draw_at_the_ends_of_the_uniforms(A, dev):
     """u = 0 takes the first kept action, the largest u the last; what lies outside [0, 1) counts as its nearest end"""
     from parl_amd import ops
-    x = _logits(6, 3000, torch.float32, dev, 1)
+    x = _logits(6, A, torch.float32, dev, 1)
     x[:, :5] = float('-inf')
     u = torch.tensor([0.0, 1.0 - 2.0**-53, -3.0, 1.0, 7.0, float('nan')], dtype=torch.float64, device=dev)
     for s in (dict(), dict(top_k=20), dict(top_p=0.4)):
@@ -177,9 +233,10 @@ def test_draw_at_the_ends_of_the_uniforms(dev):
         check_draw(x, v, a, lp, **s)
 
 
-def test_settings_out_of_range_in_tensors_count_as_the_nearest_end(dev):
+@pytest.mark.parametrize('A', [40, 800, 9000])
+def test_settings_out_of_range_in_tensors_count_as_the_nearest_end(A, dev):
     from parl_amd import ops
-    x = _logits(6, 800, torch.float32, dev, 2)
+    x = _logits(6, A, torch.float32, dev, 2)
     u = torch.rand(6, generator=torch.Generator(device=dev).manual_seed(3), dtype=torch.float64, device=dev)
     f = lambda *v: torch.tensor(v, device=dev)  # noqa: E731
     nan, inf = float('nan'), float('inf')
@@ -190,10 +247,10 @@ def test_settings_out_of_range_in_tensors_count_as_the_nearest_end(dev):
     # an endless temperature: every legal action alike
     x[:, 3] = -inf
     a, lp = ops.logits_sample(x, u, temperature=torch.full((6, ), inf, device=dev))
-    legal = [i for i in range(800) if i != 3]
+    legal = [i for i in range(A) if i != 3]
     for r in range(6):
-        assert int(a[r]) == legal[int(float(u[r]) * 799)]
-        assert float(lp[r]) == pytest.approx(-math.log(799), rel=1e-6)
+        assert int(a[r]) == legal[int(float(u[r]) * (A - 1))]
+        assert float(lp[r]) == pytest.approx(-math.log(A - 1), rel=1e-6)
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
