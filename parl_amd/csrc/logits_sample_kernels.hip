@@ -12,7 +12,7 @@
 // kernel below draw the same action from the same row.  (Sums in float32 would move the draw of about one row in a
 // hundred over 131,072 actions: the border between two actions has to be right to far less than their weights.)
 //
-// No sort.  Rows of at most 64 actions take lanes of a wave.  Longer rows:
+// No sort.  Rows of at most 64 actions (512 where nothing has to be ranked) lie in the registers of a wave.  Longer rows:
 //   no filter   one pass: every wave sums the weights of 4 KB at a time relative to their own maximum; the sums are brought
 //               to the row's maximum, the piece that the draw falls into is found among them and scanned.
 //   filters     what they keep is "larger than a cut value, and the first few that equal it".  One pass for the maximum,
@@ -39,7 +39,7 @@ constexpr double kFloorLog2 = -42.0;     // weights under 2^-42 are 0
 constexpr int kBins = 256;
 constexpr double kPerHalving = 6.0;
 constexpr int kLastBin = 252;            // 42 halvings
-constexpr int kMaxParts = 64;       // of a row that several workgroups share
+constexpr int kMaxParts = 64;            // segments of a row
 
 // Running sums over the lanes of a wave, by the data-parallel moves of the vector unit (a shuffle goes through LDS and takes
 // several times as long): within rows of 16 lanes, then the rows' last lanes into the rows behind them.
