@@ -26,7 +26,7 @@
 //
 // Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 101 us, 55 us of which the 268 MB
 // would take; the pass is bound by the vector unit, which issues in 89 % of its slots, 25 instructions a value.  1,024 x 100,003
-// with top-p 0.95: 31 us for the maxima (HBM), 103 for the classes (28 instructions a value), 92 for the finish
+// with top-p 0.95: 31 us for the maxima (HBM), 87 for the classes (24 instructions a value), 92 for the finish
 // (a pass over the row by each workgroup, and the chain of scans behind it).  One row of 131,072 with top-k and
 // top-p: 25 us, three launches and the finish's chain of 13 us.
 #include "common.hpp"
@@ -127,8 +127,8 @@ __device__ __forceinline__ double log2_weight(float x, float m, double c) { retu
 // |r| <= 1/2 with q the interpolation of (2^r - 1) / r at seven Chebyshev nodes: relative error 1.1e-10, and 2^0 is 1.
 // (The error is a function of r alone, so most of it cancels between a running sum and the whole: over 131,072 actions a
 // border moves by some 1e-13 of the mass.)  Adding 2^52 to a number below it leaves its nearest integer in the low bits.  No
-// branch: the weights of a load are formed side by side, 15 instructions of the vector unit each; float64 runs at
-// float32's rate here.
+// branch: the weights of a load are formed side by side, 15 instructions of the vector unit each (13 where the caller knows
+// that y >= -42: CHECK false); float64 runs at float32's rate here.
 // a b + c with c in scalar registers: left to itself the compiler copies the constant into the result's registers first, one
 // instruction more for every step
 __device__ __forceinline__ double fma_const(double a, double b, double c) {
@@ -137,8 +137,9 @@ __device__ __forceinline__ double fma_const(double a, double b, double c) {
   return d;
 }
 constexpr uint64_t kUnitsBase = 0x4330000000000000ULL;
+template <bool CHECK = true>
 __device__ __forceinline__ uint64_t weight_bits(double y, int shift) {
-  y = fmax(y, -1000.0);   // -inf: no NaN below
+  if constexpr (CHECK) y = fmax(y, -1000.0);   // -inf: no NaN below
   // adding 1.5 * 2^52 rounds to an integer, which then is the low word: n + shift + 1023, the exponent of the weight
   const double magic = 0x1.8p52 + (shift + 1023), t = y + magic, r = y - (t - magic);
   double p = 0x1.00a581594758ep-16;
@@ -149,7 +150,7 @@ __device__ __forceinline__ uint64_t weight_bits(double y, int shift) {
   p = fma_const(p, r, 0x1.ebfbe045f4d3cp-3);
   p = fma_const(p, r, 0x1.62e42fefa39efp-1);
   p = __builtin_fma(p, r, 1.0);
-  const double scale = __hiloint2double(y >= kFloorLog2 ? __double2loint(t) << 20 : 0, 0);   // 2^(n + shift)
+  const double scale = __hiloint2double(!CHECK || y >= kFloorLog2 ? __double2loint(t) << 20 : 0, 0);   // 2^(n + shift)
   return (uint64_t)__double_as_longlong(__builtin_fma(p, scale, 0x1p52));
 }
 __device__ __forceinline__ uint64_t weight_units(double y, int shift) { return weight_bits(y, shift) - kUnitsBase; }
@@ -509,18 +510,14 @@ __device__ __forceinline__ void add_classes(const T* __restrict__ x, int begin, 
                                             uint64_t* mass, uint32_t* count, bool counts) {
   constexpr int V = Vec16<T>::n;
   for_each_vec<T, NT>(x, begin, end, threadIdx.x, [&](const float (&v)[V], int) {
-    uint64_t u[V];
     double y[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      y[j] = log2_weight(v[j], m, r.c);
-      u[j] = weight_units(y[j], shift);
-    }
+    for (int j = 0; j < V; ++j) y[j] = log2_weight(v[j], m, r.c);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      if (y[j] >= kFloorLog2) {
+      if (y[j] >= kFloorLog2) {   // the additions need the branch; with the weight inside it the registers allow twice the waves
         const int b = weight_bin(y[j]);
-        atomicAdd((unsigned long long*)&mass[b], (unsigned long long)u[j]);
+        atomicAdd((unsigned long long*)&mass[b], (unsigned long long)(weight_bits<false>(y[j], shift) - kUnitsBase));
         if (counts) atomicAdd(&count[b], 1u);
       }
     }
