@@ -26,7 +26,7 @@
 //
 // Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 101 us, 55 us of which the 268 MB
 // would take; the pass is bound by the vector unit, which issues in 89 % of its slots, 25 instructions a value.  1,024 x 100,003
-// with top-p 0.95: 31 us for the maxima (HBM), 87 for the classes (24 instructions a value), 92 for the finish
+// with top-p 0.95: 31 us for the maxima (HBM), 83 for the classes (24 instructions a value), 92 for the finish
 // (a pass over the row by each workgroup, and the chain of scans behind it).  One row of 131,072 with top-k and
 // top-p: 25 us, three launches and the finish's chain of 13 us.
 #include "common.hpp"
