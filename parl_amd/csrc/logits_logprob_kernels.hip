@@ -78,6 +78,9 @@ __device__ __forceinline__ void stat_join_lanes(Stat& a, float c) {
   }
 }
 
+// nothing was added but -inf: a NaN alone leaves no maximum either, but makes the sum NaN
+__device__ __forceinline__ bool nothing_legal(float m, float s) { return m == -INFINITY && s == 0.f; }
+
 // the action of a row: -1 (no decision); an index outside [-1, A) is clamped and raises the data-error flag
 __device__ __forceinline__ int64_t row_action(const int64_t* __restrict__ actions, int64_t row, int64_t A, int* err) {
   int64_t a = actions[row];
@@ -93,7 +96,7 @@ __device__ __forceinline__ void row_finish(const Stat& st, const T* __restrict__
                                            float* __restrict__ log_probs, float* __restrict__ entropies,
                                            float2* __restrict__ stats) {
   float lp = 0.f, h = 0.f;
-  if (a >= 0 && st.m != -INFINITY) {
+  if (a >= 0 && !nothing_legal(st.m, st.s)) {
     const float log2s = __builtin_amdgcn_logf(st.s);
     lp = (to_f32(x[a]) - st.m) * inv_t - kLn2 * log2s;   // not in units of log 2: the lowest float stays finite
     h = kLn2 * (log2s - st.t / st.s);
@@ -220,7 +223,7 @@ __device__ __forceinline__ GradRow grad_row(const int64_t* __restrict__ actions,
   GradRow r;
   const float2 st = stats[row];
   r.a = row_action(actions, row, A, nullptr);   // the forward pass raised the flag
-  r.live = r.a >= 0 && st.x != -INFINITY;
+  r.live = r.a >= 0 && !nothing_legal(st.x, st.y);
   const float gl = g_logp ? g_logp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
   r.m = st.x;
   r.log2s = __builtin_amdgcn_logf(st.y);

@@ -416,6 +416,23 @@ def test_log_prob_of_masked_and_bad_rows(A, dtype, dev):
     assert ops.consume_device_errors() == 0
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('A', [1, 6, 100, 500, 3000, 50000])
+def test_log_prob_of_rows_without_any_number_but_nan_is_nan(A, dtype, dev):
+    """a network that has diverged: no maximum, as in an empty row, but not ignored as one"""
+    from parl_amd import ops
+    x = _logits(4, A, dtype, dev, A)
+    x[1] = float('nan')
+    x[2, 1:] = float('-inf')
+    x[2, 0] = float('nan')
+    x[3] = float('-inf')
+    x = x.requires_grad_(True)
+    lp, ent = ops.logits_log_prob(x, torch.zeros(4, dtype=torch.int64, device=dev))
+    grad, = torch.autograd.grad((lp, ent), (x, ), (torch.ones_like(lp), torch.ones_like(ent)))
+    for t in (lp, ent, grad):
+        assert torch.isfinite(t[0]).all() and torch.isnan(t[1:3]).all() and (t[3] == 0).all()
+
+
 @pytest.mark.parametrize('A', [6, 3000])
 def test_log_prob_of_an_action_outside_the_set_is_clamped_and_flagged(A, dev):
     from parl_amd import ops
