@@ -329,6 +329,10 @@ constexpr int64_t kMaxWaveRow = 4096;   // one wave per row up to here
 // of 131,072 bf16 take 613 / 594 / 579 us with 256 / 512 / 1,024 threads (both passes), 2,048 of 32,003 take 92 / 90 / 105.
 constexpr int64_t kRow512 = 16384, kRow1024 = 65536;
 
+static int row_threads(int64_t A, int64_t part) {
+  return A <= kMaxWaveRow ? 64 : part < kRow512 ? 256 : part < kRow1024 ? 512 : 1024;
+}
+
 template <typename T>
 static int logprob_forward(const T* logits, int64_t stride, const int64_t* actions, float* log_probs, float* entropies,
                            float2* stats, Stat* parts, int64_t N, int64_t A, float c, float inv_t, hipStream_t s) {
@@ -348,13 +352,14 @@ static int logprob_forward(const T* logits, int64_t stride, const int64_t* actio
   }
   const LogprobPlan p = logprob_plan(N, A);
   const int grid = (int)(N * p.n_parts);
-  if (A <= kMaxWaveRow)
+  const int threads = row_threads(A, p.part);
+  if (threads == 64)
     logprob_row_kernel<T, 64><<<grid, 64, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts, N, A,
                                                   p.n_parts, p.part, c, inv_t, err);
-  else if (p.part < kRow512)
+  else if (threads == 256)
     logprob_row_kernel<T, 256><<<grid, 256, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts,
         N, A, p.n_parts, p.part, c, inv_t, err);
-  else if (p.part < kRow1024)
+  else if (threads == 512)
     logprob_row_kernel<T, 512><<<grid, 512, 0, s>>>(logits, stride, actions, log_probs, entropies, stats, parts,
         N, A, p.n_parts, p.part, c, inv_t, err);
   else
@@ -384,13 +389,14 @@ static int logprob_backward(const T* logits, int64_t stride, const int64_t* acti
   }
   const LogprobPlan p = logprob_plan(N, A);
   const int grid = (int)(N * p.n_parts);
-  if (A <= kMaxWaveRow)
+  const int threads = row_threads(A, p.part);
+  if (threads == 64)
     logprob_row_grad_kernel<T, 64><<<grid, 64, 0, s>>>(logits, stride, actions, stats, entropies, g_logp, g_ent, grad, A,
                                                        p.n_parts, p.part, c, inv_t);
-  else if (p.part < kRow512)
+  else if (threads == 256)
     logprob_row_grad_kernel<T, 256><<<grid, 256, 0, s>>>(logits, stride, actions, stats, entropies, g_logp,
         g_ent, grad, A, p.n_parts, p.part, c, inv_t);
-  else if (p.part < kRow1024)
+  else if (threads == 512)
     logprob_row_grad_kernel<T, 512><<<grid, 512, 0, s>>>(logits, stride, actions, stats, entropies, g_logp,
         g_ent, grad, A, p.n_parts, p.part, c, inv_t);
   else
@@ -405,8 +411,11 @@ static int logprob_check(const void* logits, int dtype, int64_t stride, const in
   if (!(temperature > 0.f) || !(temperature < INFINITY) || !(kLog2e / temperature < INFINITY)) return PARLHIP_EINVAL;
   if (dtype != PARLHIP_F32 && dtype != PARLHIP_BF16 && dtype != PARLHIP_F16) return PARLHIP_ENOSUP;
   if (A > ((int64_t)1 << 31) || N > ((int64_t)1 << 40) / A) return PARLHIP_ENOSUP;
-  if (A > kMaxSmall && N * logprob_plan(N, A).n_parts > 0xffffffffLL / 256) return PARLHIP_ENOSUP;   // one launch's threads
   if (N == 0) return PARLHIP_OK;
+  if (A > kMaxSmall) {
+    const LogprobPlan p = logprob_plan(N, A);
+    if (N * p.n_parts > 0xffffffffLL / row_threads(A, p.part)) return PARLHIP_ENOSUP;   // one launch's threads
+  }
   if (!logits || !actions) return PARLHIP_EINVAL;
   if (reinterpret_cast<uintptr_t>(logits) & (dtype == PARLHIP_F32 ? 3 : 1)) return PARLHIP_EINVAL;
   return PARLHIP_OK;

@@ -72,6 +72,26 @@ def test_log_prob_arguments(lib):
     assert lib.parlhip_logits_log_prob_workspace_bytes(5, 6) == 0
 
 
+@pytest.mark.parametrize('A', [1, 512, 513, 4096, 5000, 131072])
+def test_log_prob_of_no_rows_and_of_more_than_a_launch_takes(lib, A):
+    f = lambda N: lib.parlhip_logits_log_prob(None, 0, A, None, None, None, None, N, A, 1.0, None, 0, None)  # noqa: E731
+    b = lambda N: lib.parlhip_logits_log_prob_backward(None, 0, A, None, None, None, None, None, None, N, A, 1.0,  # noqa: E731
+                                                       None)
+    assert f(0) == 0 and b(0) == 0
+    # a launch has fewer than 2^32 threads; up to 512 actions it walks over the rows
+    threads = None if A <= 512 else 64 if A <= 4096 else 256 if A < 16384 else 1024
+    if threads:
+        most = 0xffffffff // threads
+        assert f(most + 1) == NOSUP and b(most + 1) == NOSUP
+        if most * A <= 1 << 40:
+            assert f(most) == INVALID and b(most) == INVALID   # the NULL pointers
+
+
+def test_log_prob_of_more_rows_than_a_launch_of_512_threads_takes(lib):
+    f = lambda N: lib.parlhip_logits_log_prob(None, 0, 16384, None, None, None, None, N, 16384, 1.0, None, 0, None)  # noqa: E731
+    assert f(0xffffffff // 512) == INVALID and f(0xffffffff // 512 + 1) == NOSUP
+
+
 def test_grad_norm_arguments(lib):
     def arr(t, *v):
         return (t * len(v))(*v)
