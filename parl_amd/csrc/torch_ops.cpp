@@ -93,7 +93,7 @@ Rows rows_of(const Tensor& logits) {
   Rows r;
   r.a = logits.size(-1);
   r.n = logits.numel() / r.a;
-  r.x = logits.detach();
+  r.x = logits.detach().resolve_neg();
   if (r.x.dim() != 2) r.x = r.x.reshape({r.n, r.a});
   r.stride = r.n > 1 ? r.x.stride(0) : r.a;
   if (r.stride < r.a || (r.a > 1 && r.x.stride(1) != 1)) {
@@ -108,7 +108,7 @@ Tensor per_row(const Tensor& t, at::ScalarType dtype, const Tensor& logits, cons
   if (t.device() != logits.device()) refuse(name, ": ", what, " is on ", t.device(), ", logits on ", logits.device());
   const at::IntArrayRef lead = logits.sizes().slice(0, logits.dim() - 1);
   if (t.sizes() != lead) refuse(name, ": ", what, " must have the shape ", lead, ", got ", t.sizes());
-  return t.detach().contiguous();
+  return t.detach().resolve_neg().contiguous();
 }
 
 Tensor unpack(const py::handle& h, const char* what, const char* name) {
@@ -209,7 +209,7 @@ struct LogProbFn : torch::autograd::Function<LogProbFn> {
     const c10::DeviceGuard guard(logits.device());
     const Rows r = rows_of(logits);
     for (Tensor& t : g)
-      if (t.defined()) t = t.to(at::kFloat).contiguous();
+      if (t.defined()) t = t.to(at::kFloat).resolve_neg().contiguous();
     const Tensor grad = at::empty(logits.sizes(), logits.options());
     check(lib.log_prob_backward(data(r.x), type_code(logits), r.stride, (const int64_t*)data(actions),
                                 (const float*)data(stats), (const float*)data(entropies), (const float*)data(g[0]),
@@ -248,6 +248,7 @@ struct Table {
       refuse(name, ": needs dense float32, bfloat16 or float16 tensors, got ", t.layout(), " ", t.scalar_type());
     if (!t.is_cuda() || (device && t.device() != *device))
       refuse(name, ": the tensors must be on one HIP device, got ", t.device());
+    if (t.is_neg()) refuse(name, ": a lazily negated view has no values in memory to read or write");
     if (!t.is_non_overlapping_and_dense())
       refuse(name, ": a tensor of shape ", t.sizes(), " and strides ", t.strides(), " does not fill its memory");
     device = t.device();
@@ -311,7 +312,11 @@ Tensor clip_grad_norm(const py::handle& parameters, double max_norm, bool error_
     }
   }
   if (error_if_nonfinite) {
-    const double norm = run_norm(g).item<double>();
+    double norm;
+    {
+      py::gil_scoped_release free;   // waits for the device
+      norm = run_norm(g).item<double>();
+    }
     if (!std::isfinite(norm)) {
       std::ostringstream s;
       s << name << ": the global norm of the gradients is " << norm << "; they are unchanged";

@@ -196,6 +196,15 @@ def test_refusals(dev):
     assert float(ops.grad_norm([shared, shared])) == pytest.approx(math.sqrt(200))   # reading twice is no conflict
 
 
+def test_a_lazily_negated_view_is_refused(dev):
+    from parl_amd import ops
+    from parl_amd._native import ParlHipError
+    v = torch.view_as_complex(torch.ones(1, 2, device=dev)).conj().imag   # one element: dense for all its stride of two
+    assert v.is_neg()
+    with pytest.raises(ParlHipError, match='negated'):
+        ops.grad_norm([v])
+
+
 @pytest.mark.parametrize('n', [10, 200])
 def test_clip_in_replayed_graphs_and_on_two_streams(n, dev):
     from parl_amd import ops

@@ -476,6 +476,43 @@ def test_log_prob_of_no_rows(dev):
     assert lp.shape == (0, ) and x.grad.shape == (0, 9)
 
 
+def test_lazily_negated_views_are_read_as_what_they_are(dev):
+    """the imaginary part of a conjugate: a view whose memory holds the values with the other sign"""
+    from parl_amd import ops
+
+    def pair(*shape, dtype=torch.float32):
+        t = torch.randn(*shape, 2, dtype=dtype, device=dev)
+        v = torch.view_as_complex(t).conj().imag
+        assert v.is_neg()
+        return v, -t[..., 1]
+
+    x, x0 = pair(20, 33)
+    y, y0 = pair(20, 33, 1)
+    u, u0 = pair(20, dtype=torch.float64)
+    a = torch.randint(0, 33, (20, ), device=dev)
+    for v, v0 in ((x, x0), (y[..., 0], y0[..., 0])):
+        for got, want in zip(ops.logits_sample(v, u), ops.logits_sample(v0.contiguous(), u0.contiguous())):
+            assert torch.equal(got, want)
+    leaf, leaf0 = x.detach().requires_grad_(True), x0.contiguous().requires_grad_(True)
+    g, g0 = pair(20)
+    out, out0 = ops.logits_log_prob(leaf, a), ops.logits_log_prob(leaf0, a)
+    assert torch.equal(out[0], out0[0]) and torch.equal(out[1], out0[1])
+    assert torch.equal(torch.autograd.grad(out, (leaf, ), (g, g))[0],
+                       torch.autograd.grad(out0, (leaf0, ), (g0.contiguous(), g0.contiguous()))[0])
+
+
+@pytest.mark.parametrize('lead', [(0, ), (3, 0)])
+@pytest.mark.parametrize('A', [1, 9, 600, 5000, 131072])
+def test_no_rows_of_any_length(A, lead, dev):
+    from parl_amd import ops
+    x = torch.empty(*lead, A, device=dev, requires_grad=True)
+    a, lp0 = ops.logits_sample(x, torch.empty(lead, dtype=torch.float64, device=dev), top_p=0.9)
+    assert a.shape == lead and lp0.shape == lead
+    lp, ent = ops.logits_log_prob(x, a)
+    (lp.sum() + ent.sum()).backward()
+    assert lp.shape == lead and ent.shape == lead and x.grad.shape == x.shape
+
+
 def test_log_prob_gradient_matches_differences(dev):
     """central differences of the float64 formula at the kernel's own gradient"""
     x = _logits(3, 11, torch.float32, dev, 5, spread=1.0)
