@@ -10,11 +10,13 @@
 // Every sum is an INTEGER: w is formed in float64 and rounded once to a multiple of 2^-s (s = 44 for A = 2^18, more for
 // fewer actions), so a sum is the same in any order and in any split over threads, atomics included, and the forms of this
 // kernel below draw the same action from the same row.  (Sums in float32 would move the draw of about one row in a
-// hundred over 131,072 actions: the border between two actions has to be right to far less than their weights.)
+// hundred over 131,072 actions: the border between two actions has to be right to far less than their weights.)  So every
+// form reads the row for its maximum before it forms a weight.  Sums of stretches relative to their own maxima would need
+// no such pass, but count what is under 2^-42 of the row's largest, and round every weight at another place.
 //
 // No sort.  Rows of at most 64 actions (512 where nothing has to be ranked) lie in the registers of a wave.  Longer rows:
-//   no filter   one pass: every wave sums the weights of 4 KB at a time relative to their own maximum; the sums are brought
-//               to the row's maximum, the piece that the draw falls into is found among them and scanned.
+//   no filter   one pass for the maximum of every 4 KB, one in which every wave sums the weights of 4 KB at a time; the piece
+//               that the draw falls into is found among the sums and scanned.
 //   filters     what they keep is "larger than a cut value, and the first few that equal it".  One pass for the maximum,
 //               one that adds masses (and counts, for top-k) into 256 classes of -log2 w, for each segment of the
 //               row; the class that holds the border is found by a scan and taken apart on a list of its
@@ -24,11 +26,12 @@
 // Rows of up to 4,096 actions do that in one wave each.  Above, every pass over the rows is a launch of its own over segments of
 // all rows, which fills the card whether the rows are many or few and long, and a workgroup per row finishes.
 //
-// Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 101 us, 55 us of which the 268 MB
-// would take; the pass is bound by the vector unit, which issues in 89 % of its slots, 25 instructions a value.  1,024 x 100,003
-// with top-p 0.95: 31 us for the maxima (HBM), 83 for the classes (24 instructions a value), 92 for the finish
-// (a pass over the row by each workgroup, and the chain of scans behind it).  One row of 131,072 with top-k and
-// top-p: 27 us, three launches of 4, 7 and 14, the last a chain of scans.
+// Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 144 us, 55 us of which one read of
+// the 268 MB would take: 38 for the maxima (HBM and cache), 100 for the masses (the vector unit, 25 instructions a value), 8 for
+// the finish.  Sums relative to the pieces' own maxima, in one pass, took 110 and were another distribution (above).
+// 1,024 x 100,003 with top-p 0.95: 31 us for the maxima, 84 for the classes (24 instructions a value), 92 for the finish
+// (a pass over the row by each workgroup, and the chain of scans behind it), 212 with what lies between them.  One row of
+// 131,072 with top-k and top-p: 27 us, three launches of 4, 7 and 14, the last a chain of scans.
 #include "common.hpp"
 #include "logits_common.hpp"
 
@@ -36,6 +39,7 @@ namespace parlhip {
 
 constexpr int64_t kSampleMaxActions = (int64_t)1 << 20;
 constexpr double kFloorLog2 = -42.0;     // weights under 2^-42 are 0
+constexpr float kFloor = 0x1p-42f;
 constexpr int kBins = 256;
 constexpr double kPerHalving = 6.0;
 constexpr int kLastBin = 252;            // 42 halvings
@@ -104,12 +108,15 @@ __device__ __forceinline__ Row row_settings(const SampleArgs& q, int64_t row) {
   if (r.top_p == 0.f) r.k = 1;            // only the first action
   if (r.k == 1) r.top_p = 1.f;
   r.c = 1.4426950408889634 / (double)t;
-  r.ymin = min_p > 0.f ? fmax(kFloorLog2, log2((double)min_p)) : kFloorLog2;
+  r.ymin = min_p > kFloor ? fmax(kFloorLog2, log2((double)min_p)) : kFloorLog2;
   return r;
 }
 
 // whether anything but the maximum and the whole mass is asked for
 __device__ __forceinline__ bool filtered(const Row& r) { return !r.greedy && (r.k > 0 || r.top_p < 1.f || r.ymin > kFloorLog2); }
+
+// whether nothing but the maximum and the whole mass is
+__device__ __forceinline__ bool weighed(const Row& r) { return !r.greedy && !filtered(r); }
 
 // the order of values as unsigned integers; -0 is 0
 __device__ __forceinline__ uint32_t value_key(float x) {
@@ -357,7 +364,7 @@ __device__ __forceinline__ void for_each_vec(const T* __restrict__ x, int begin,
   }
 }
 
-// the pieces of a row whose weights are summed relative to their own maximum: what a wave loads at a time
+// the pieces of a row whose maxima and masses are kept: what a wave loads at a time
 template <typename T>
 __host__ __device__ constexpr int piece_length() { return 64 * 4 * 16 / (int)sizeof(T); }
 
@@ -438,55 +445,69 @@ __device__ __forceinline__ float maximum3(float a, float b, float c) {   // NaN 
   return __builtin_elementwise_maximum(a, __builtin_elementwise_maximum(b, c));
 }
 
-// The pieces [first, last) of a row, one after the other by each of the waves `wave` of `waves`: their maxima and, with
-// SUM, their masses relative to these.
+// piece p of a row by the lanes of a wave; -inf, which has no weight, behind the row's end
 template <typename T>
-__device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, double c, int shift, int first, int last, int wave,
-                                           int waves, const Pieces& out, bool sum) {
+__device__ __forceinline__ void load_piece(const T* __restrict__ x, int A, int p, Vec16<T> (&raw)[4]) {
   constexpr int V = Vec16<T>::n, kLen = piece_length<T>();
-  const int lane = threadIdx.x & 63;
-  for (int p = first + wave; p < last; p += waves) {
-    const int base = p * kLen + lane * V;
-    const int loads = A - p * kLen >= kLen ? 4 : (A - p * kLen + 64 * V - 1) / (64 * V);   // of the wave
-    Vec16<T> raw[4];
-    if (p * kLen + kLen <= A) {
+  const int base = p * kLen + (int)(threadIdx.x & 63) * V;
+  if (p * kLen + kLen <= A) {
 #pragma unroll
-      for (int a = 0; a < 4; ++a) raw[a].load(x + base + a * 64 * V);
+    for (int a = 0; a < 4; ++a) raw[a].load(x + base + a * 64 * V);
+    return;
+  }
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    const int i0 = base + a * 64 * V;
+    if (i0 + V <= A) {
+      raw[a].load(x + i0);
     } else {
+      float g[V];
 #pragma unroll
-      for (int a = 0; a < 4; ++a) {
-        const int i0 = base + a * 64 * V;
-        if (i0 + V <= A) {
-          raw[a].load(x + i0);
-        } else {
-          float g[V];
-#pragma unroll
-          for (int j = 0; j < V; ++j) g[j] = i0 + j < A ? to_f32(x[i0 + j]) : -INFINITY;
-          raw[a].pack(g);   // exact: they came from this type
-        }
-      }
+      for (int j = 0; j < V; ++j) g[j] = i0 + j < A ? to_f32(x[i0 + j]) : -INFINITY;
+      raw[a].pack(g);   // exact: they came from this type
     }
+  }
+}
+
+// the maxima of the pieces [first, last) of a row, one after the other by each of the waves `wave` of `waves`
+template <typename T>
+__device__ __forceinline__ void max_pieces(const T* __restrict__ x, int A, int first, int last, int wave, int waves,
+                                           float* __restrict__ max) {
+  constexpr int V = Vec16<T>::n;
+  for (int p = first + wave; p < last; p += waves) {
+    Vec16<T> raw[4];
+    load_piece(x, A, p, raw);
     float m = -INFINITY;   // a NaN stays
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int j = 0; j < V; j += 2) m = maximum3(m, raw[a].get(j), raw[a].get(j + 1));
     m = group_max<64>(m < INFINITY ? m : __builtin_nanf(""), nullptr);
-    if (sum) {
-      uint64_t mass = 0;
-      if (m > -INFINITY) {
+    if ((threadIdx.x & 63) == 0) max[p] = m;
+  }
+}
+
+// their masses, with the row's maximum m
+template <typename T>
+__device__ __forceinline__ void sum_pieces(const T* __restrict__ x, int A, float m, double c, int shift, int first, int last,
+                                           int wave, int waves, const Pieces& out) {
+  constexpr int V = Vec16<T>::n, kLen = piece_length<T>();
+  for (int p = first + wave; p < last; p += waves) {
+    const int loads = A - p * kLen >= kLen ? 4 : (A - p * kLen + 64 * V - 1) / (64 * V);   // of the wave
+    uint64_t mass = 0;
+    if (log2_weight(out.max[p], m, c) >= kFloorLog2) {   // else nothing in it has a weight
+      Vec16<T> raw[4];
+      load_piece(x, A, p, raw);
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-          if (a >= loads) break;
+      for (int a = 0; a < 4; ++a) {
+        if (a >= loads) break;
 #pragma unroll
-          for (int j = 0; j < V; ++j) mass += weight_bits(log2_weight(raw[a].get(j), m, c), shift);
-        }
-        mass -= (uint64_t)(loads * V) * kUnitsBase;
-        mass = wave_total(mass);
+        for (int j = 0; j < V; ++j) mass += weight_bits(log2_weight(raw[a].get(j), m, c), shift);
       }
-      if (lane == 0) out.mass[p] = mass;
+      mass -= (uint64_t)(loads * V) * kUnitsBase;
+      mass = wave_total(mass);
     }
-    if (lane == 0) out.max[p] = m;
+    if ((threadIdx.x & 63) == 0) out.mass[p] = mass;
   }
 }
 
@@ -860,14 +881,13 @@ __device__ __forceinline__ void sum_segments(const RowView<T>& v, RowWork<NT>& w
 }
 
 // Scans [begin, end) in index order for the first action whose running kept mass exceeds target; of the values at the cut
-// the first `left` are kept, each with `one` (0: none are).  True if it was there, else `seen` is the mass that was.
+// the first `left` are kept, each with `one` (0: none are).  It is there: the range's mass is the same sum.
 template <typename T, int NT>
-__device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row, int begin,
+__device__ __forceinline__ void scan_draw(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row, int begin,
                                           int end, const Cut& cut, uint64_t one, uint32_t left, uint64_t target,
-                                          uint64_t total, uint64_t& seen) {
+                                          uint64_t total) {
   constexpr int V = Vec16<T>::n;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  seen = 0;
   for (int base = begin; base < end; base += NT * V) {
     const int i0 = base + (int)threadIdx.x * V;
     float g[V];
@@ -936,13 +956,11 @@ __device__ __forceinline__ bool scan_draw(const RowView<T>& v, RowWork<NT>& w, c
           before += u[j];
         }
       }
-      return true;
+      return;
     }
     target -= here;
-    seen += here;
     left -= tie_all < left ? tie_all : left;
   }
-  return false;
 }
 
 // The draw of a filtered row, from its segments' classes.
@@ -977,21 +995,16 @@ __device__ __forceinline__ void draw_filtered(const RowView<T>& v, RowWork<NT>& 
   const uint32_t left = w.lo;
   const uint64_t target = w.found_target;
   const int begin = s * v.seg_len, end = begin + v.seg_len < v.A ? begin + v.seg_len : v.A;
-  uint64_t seen;
-  scan_draw(v, w, q, row, begin, end, cut, one, left, target, total, seen);
+  scan_draw(v, w, q, row, begin, end, cut, one, left, target, total);
 }
 
-// The draw of a row without filters, from the sums of its n <= NT pieces.
+// The draw of a row without filters, from the masses of its n <= NT pieces.
 template <typename T, int NT>
 __device__ __forceinline__ void draw_pieces(const RowView<T>& v, RowWork<NT>& w, const SampleArgs& q, int64_t row, const Pieces& p,
                                             int n) {
   constexpr int kLen = piece_length<T>();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = threadIdx.x;
-  const uint64_t raw = i < n ? p.mass[i] : 0;
-  const float ref = i < n ? p.max[i] : -INFINITY;
-  // the piece's mass relative to the row's maximum: exact where that is the piece's own, rounded to 53 bits elsewhere
-  const double y = ref > -INFINITY ? log2_weight(ref, v.m, v.r.c) : -1e9;
-  const uint64_t mass = y == 0.0 ? raw : y >= kFloorLog2 ? (uint64_t)rint((double)raw * exp2(y)) : 0;
+  const uint64_t mass = i < n ? p.mass[i] : 0;
   const uint64_t run = wave_scan(mass);
   uint64_t before = run - mass, total = 0;
   if constexpr (NT > 64) {
@@ -1014,11 +1027,7 @@ __device__ __forceinline__ void draw_pieces(const RowView<T>& v, RowWork<NT>& w,
   __syncthreads();
   const int begin = w.found * kLen, end = begin + kLen < v.A ? begin + kLen : v.A;
   const Cut all{-INFINITY, 0, 0};
-  uint64_t seen;
-  // The weights of the piece, each rounded relative to the row's maximum, may sum to a few units less than its mass did;
-  // its largest is at least one unit.
-  if (!scan_draw(v, w, q, row, begin, end, all, 0, 0, w.found_target, total, seen))
-    scan_draw(v, w, q, row, begin, end, all, 0, 0, seen - 1, total, seen);
+  scan_draw(v, w, q, row, begin, end, all, 0, 0, w.found_target, total);
 }
 
 // the largest logit, the first among equals
@@ -1086,11 +1095,14 @@ __global__ __launch_bounds__(64) void sample_wave_kernel(const T* __restrict__ l
   v.seg_first = nullptr;
   v.values = nullptr;
   const Pieces p{piece_mass, piece_max};
-  const bool hists = filtered(v.r);
-  sum_pieces(v.x, A, v.r.c, v.shift, 0, (A + piece_length<T>() - 1) / piece_length<T>(), 0, 1, p, !hists && !v.r.greedy);
+  const int pieces = (A + piece_length<T>() - 1) / piece_length<T>();
+  max_pieces(v.x, A, 0, pieces, 0, 1, p.max);
   __syncthreads();
   v.m = row_max<T, 64>(p, A, w.red32);
-  if (hists && v.m > -INFINITY) {
+  if (v.m > -INFINITY && weighed(v.r)) {
+    sum_pieces(v.x, A, v.m, v.r.c, v.shift, 0, pieces, 0, 1, p);
+    __syncthreads();
+  } else if (v.m > -INFINITY && filtered(v.r)) {
     for (int i = threadIdx.x; i < kBins; i += 64) { hist[i] = 0; count[i] = 0; }
     __syncthreads();
     add_classes<T, 64>(v.x, 0, A, v.m, v.r, v.shift, hist, count, v.r.k > 0);
@@ -1116,22 +1128,36 @@ struct SamplePlan {
 
 constexpr int kPartThreads = 256;
 
-// a workgroup for `per` pieces: their maxima, and their masses where that is all a row needs
+// a workgroup for `per` pieces: their maxima
 template <typename T>
-__global__ __launch_bounds__(kPartThreads) void sample_pieces_kernel(const T* __restrict__ logits, int64_t stride, int A,
+__global__ __launch_bounds__(kPartThreads) void sample_maxima_kernel(const T* __restrict__ logits, int64_t stride, int A,
+                                                                     SamplePlan plan, int64_t row0, int per) {
+  const int n = (A + piece_length<T>() - 1) / piece_length<T>();
+  const uint32_t groups = (n + per - 1) / per;
+  const int64_t row = row0 + blockIdx.x / groups;
+  const int first = (int)(blockIdx.x % groups) * per, last = first + per < n ? first + per : n;
+  max_pieces(logits + row * stride, A, first, last, threadIdx.x >> 6, kPartThreads / 64, plan.piece_max + row * plan.n_piece);
+}
+
+// a workgroup for `per` pieces: their masses, where no row has a filter
+template <typename T>
+__global__ __launch_bounds__(kPartThreads) void sample_masses_kernel(const T* __restrict__ logits, int64_t stride, int A,
                                                                      SampleArgs q, SamplePlan plan, int64_t row0, int per) {
+  __shared__ uint32_t red[kPartThreads / 64];
   const int n = (A + piece_length<T>() - 1) / piece_length<T>();
   const uint32_t groups = (n + per - 1) / per;
   const int64_t row = row0 + blockIdx.x / groups;
   const Row r = row_settings(q, row);
   const int first = (int)(blockIdx.x % groups) * per, last = first + per < n ? first + per : n;
   const Pieces p{plan.piece_mass + row * plan.n_piece, plan.piece_max + row * plan.n_piece};
-  sum_pieces(logits + row * stride, A, r.c, q.shift, first, last, threadIdx.x >> 6, kPartThreads / 64, p,
-             !r.greedy && !filtered(r));
+  const float m = row_max<T, kPartThreads>(p, A, red);
+  if (m > -INFINITY)
+    sum_pieces(logits + row * stride, A, m, r.c, q.shift, first, last, threadIdx.x >> 6, kPartThreads / 64, p);
 }
 
-// a workgroup per segment: its classes, where the row has filters
-template <typename T>
+// A workgroup per segment: its classes, where the row has filters.  MIXED: the settings are each row's own, and where they
+// are no filters the segment's pieces are summed.
+template <typename T, bool MIXED>
 __global__ __launch_bounds__(kPartThreads) void sample_classes_kernel(const T* __restrict__ logits, int64_t stride, int A,
                                                                       SampleArgs q, SamplePlan plan, int64_t row0) {
   __shared__ uint64_t hist[kBins];
@@ -1139,10 +1165,18 @@ __global__ __launch_bounds__(kPartThreads) void sample_classes_kernel(const T* _
   const int64_t row = row0 + blockIdx.x / plan.n_seg;
   const int seg = blockIdx.x % plan.n_seg;
   const Row r = row_settings(q, row);
-  if (!filtered(r)) return;
-  const Pieces p{nullptr, plan.piece_max + row * plan.n_piece};
+  if (MIXED ? r.greedy : !filtered(r)) return;
+  const Pieces p{plan.piece_mass + row * plan.n_piece, plan.piece_max + row * plan.n_piece};
   const float m = row_max<T, kPartThreads>(p, A, red);
   if (!(m > -INFINITY)) return;
+  if constexpr (MIXED) {
+    if (weighed(r)) {
+      const int n = (A + piece_length<T>() - 1) / piece_length<T>(), of = plan.seg_len / piece_length<T>();   // exact
+      const int first = seg * of, last = first + of < n ? first + of : n;
+      sum_pieces(logits + row * stride, A, m, r.c, q.shift, first, last, threadIdx.x >> 6, kPartThreads / 64, p);
+      return;
+    }
+  }
   static_assert(kPartThreads == kBins, "a thread for each class");
   const int b = threadIdx.x;
   hist[b] = 0;
@@ -1270,20 +1304,23 @@ static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, con
   const SamplePlan p = sample_plan(B, A, workspace);
   const bool per_row = q.temperature || q.top_k || q.top_p || q.min_p;
   const bool greedy = !per_row && q.temperature_s == 0.f;
-  const bool filters = per_row || (!greedy && (q.top_k_s > 0 || q.top_p_s < 1.f || q.min_p_s > 0.f));
+  const bool filters = per_row || (!greedy && (q.top_k_s > 0 || q.top_p_s < 1.f || q.min_p_s > kFloor));   // as filtered()
   const int64_t group = filters ? p.group : B;
   for (int64_t row0 = 0; row0 < B; row0 += group) {
     const int64_t rows = row0 + group < B ? group : B - row0;
     // a piece for each wave, or two where that makes more than enough workgroups
     const int pieces = (int)((A + piece_length<T>() - 1) / piece_length<T>());
     const int per = rows * pieces >= 65536 ? 8 : 4;
-    sample_pieces_kernel<T><<<(int)(rows * ((pieces + per - 1) / per)), kPartThreads, 0, s>>>(logits, stride, (int)A, q, p,
-                                                                                            row0, per);
+    const int groups = (int)(rows * ((pieces + per - 1) / per));
+    sample_maxima_kernel<T><<<groups, kPartThreads, 0, s>>>(logits, stride, (int)A, p, row0, per);
     if (int rc = check_launch()) return rc;
-    if (filters) {
-      sample_classes_kernel<T><<<(int)(rows * p.n_seg), kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
-      if (int rc = check_launch()) return rc;
-    }
+    if (per_row)
+      sample_classes_kernel<T, true><<<(int)(rows * p.n_seg), kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    else if (filters)
+      sample_classes_kernel<T, false><<<(int)(rows * p.n_seg), kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0);
+    else if (!greedy)
+      sample_masses_kernel<T><<<groups, kPartThreads, 0, s>>>(logits, stride, (int)A, q, p, row0, per);
+    if (int rc = check_launch()) return rc;
     // a thread for each piece of a row; else smaller workgroups, more rows side by side, where the rows are many
     if (pieces > 512)
       sample_finish_kernel<T, 1024><<<(int)rows, 1024, 0, s>>>(logits, stride, (int)A, q, p, row0);

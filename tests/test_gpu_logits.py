@@ -614,3 +614,53 @@ def test_calls_on_two_streams_and_in_a_replayed_graph(A, dev):
             step(xs[0], us[0])
             torch.cuda.synchronize()
             assert all(torch.equal(p, q) for p, q in zip(full[j], outs[i]))
+
+
+# -------------------------------------------------------------------------------- one definition in every form
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('A', [600, 4096, 5000, 20000, 131072, 1 << 20])
+def test_a_weight_under_the_floor_counts_nothing(A, dtype, dev):
+    """Rows full of values just under 2^-42 of the largest, one just above it in every thousand: those under it are no choice
+    and no part of the mass, with a filter that keeps everything, without one, and in any type."""
+    from parl_amd import ops
+    x = torch.full((12, A), -29.125, dtype=dtype, device=dev)   # 2^-42.08; exact in every type
+    x[:, ::1000] = -29.0                                         # 2^-41.9
+    x[8:, ::1000] = -29.125                                      # nothing but the largest
+    x[:4, -1], x[4:8, 0], x[8:, A // 2] = 0.0, 0.0, 0.0
+    t = float(np.float32(29.0 / math.log(2.0) / 41.9))
+    few = A * 2.0**-42.08                                        # what the values under the floor would add up to
+    u = torch.tensor([0.0, 0.2 * few, 0.5 * few, 0.5] * 3, dtype=torch.float64, device=dev)
+    a, lp = ops.logits_sample(x, u, temperature=t)
+    xs, us = x.double().cpu().numpy(), u.cpu().numpy()
+    bits = math.ceil(math.log2(A))
+    for r in range(12):
+        want, want_lp = draw_row(xs[r], us[r], t, 0, 1.0, 0.0)
+        assert int(a[r]) == want, 'row %d' % r
+        # each of the n weights is off by at most half a unit of 2^-min(51, 62 - bits), the logarithm rounded once
+        n = -(-A // 1000)
+        assert float(lp[r]) == pytest.approx(want_lp, rel=2.0**-23, abs=n * 2.0**-(min(51, 62 - bits) + 1) + 1e-15), 'row %d' % r
+    k = torch.zeros(12, dtype=torch.int32, device=dev)
+    k[::2] = A
+    for y, kw in ((x, dict(top_k=A)), (x, dict(top_k=k)), (x.float(), dict()), (x.float(), dict(top_k=A))):
+        b, lq = ops.logits_sample(y, u, temperature=t, **kw)
+        assert torch.equal(a, b) and torch.equal(lp, lq), kw
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('A', [18, 64, 300, 700, 4096, 4097, 40000, 131072])
+def test_a_filter_that_keeps_everything_changes_nothing(A, dtype, dev):
+    """top-k of all actions, a minimum that none is under, float32 copies of 16-bit rows: the same bits"""
+    from parl_amd import ops
+    rows = 48
+    x = _logits(rows, A, dtype, dev, A, spread=4.0)
+    x[::5, ::3] = float('-inf')
+    x[7] = float('-inf')
+    u = torch.rand(rows, generator=torch.Generator(device=dev).manual_seed(A), dtype=torch.float64, device=dev)
+    a, lp = ops.logits_sample(x, u, temperature=0.8)
+    k = torch.zeros(rows, dtype=torch.int32, device=dev)
+    k[::2] = A
+    for y, kw in ((x, dict(top_k=A)), (x, dict(top_k=k)), (x, dict(min_p=2.0**-44)), (x.float(), dict()), (x.float(), dict(top_k=A))):
+        b, lq = ops.logits_sample(y, u, temperature=0.8, **kw)
+        assert torch.equal(a, b) and torch.equal(lp, lq), kw
