@@ -635,8 +635,8 @@ int parlhip_clip_adam_f32(int n_tensors, float* const* params, float* const* gra
  * A row whose every logit is -inf gives action -1 and log_prob 0.  A row with a NaN or +inf gives action -1 and log_prob NaN
  * and raises the data-error flag (parlhip_consume_device_errors); the other rows are not touched by it.
  * Sums are integers (multiples of 2^-42 of the row's largest weight or finer), so the draw does not depend on how
- * the work is split.  A <= 2^20 (else PARLHIP_ENOSUP).  workspace: parlhip_logits_sample_workspace_bytes(B, A) bytes,
- * 8-byte aligned (may be NULL when that is 0).                                                                     */
+ * the work is split.  A <= 2^20; B <= 2^26 - 4 up to 4,096 actions, B * A <= 2^40 above (else PARLHIP_ENOSUP).
+ * workspace: parlhip_logits_sample_workspace_bytes(B, A) bytes, 8-byte aligned (may be NULL when that is 0).           */
 size_t parlhip_logits_sample_workspace_bytes(int64_t B, int64_t A);
 int parlhip_logits_sample(const void* logits, int dtype, int64_t row_stride, const double* uniforms,
                           const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,

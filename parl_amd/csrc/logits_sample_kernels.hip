@@ -34,6 +34,7 @@
 // 131,072 with top-k and top-p: 27 us, three launches of 4, 7 and 14, the last a chain of scans.
 #include "common.hpp"
 #include "logits_common.hpp"
+#include <algorithm>
 
 namespace parlhip {
 
@@ -1243,7 +1244,7 @@ static inline int sample_shift(int64_t A) {
 static SamplePlan sample_plan(int64_t B, int64_t A, void* workspace) {
   constexpr int64_t kPiece = piece_length<float>();   // the shorter ones
   SamplePlan p;
-  p.group = ((int64_t)256 << 20) / A;                 // 100 MB of classes
+  p.group = ((int64_t)256 << 20) / A;                 // 100 MB of classes, 201 where a row is little more than a segment
   if (p.group < 1) p.group = 1;
   if (p.group > B) p.group = B;
   // segments of about 8,192 actions (the last pass scans one of them), of fewer where the rows are few
@@ -1305,11 +1306,13 @@ static int sample_run(const T* logits, int64_t stride, int64_t B, int64_t A, con
   const bool per_row = q.temperature || q.top_k || q.top_p || q.min_p;
   const bool greedy = !per_row && q.temperature_s == 0.f;
   const bool filters = per_row || (!greedy && (q.top_k_s > 0 || q.top_p_s < 1.f || q.min_p_s > kFloor));   // as filtered()
-  const int64_t group = filters ? p.group : B;
+  const int pieces = (int)((A + piece_length<T>() - 1) / piece_length<T>());
+  // a launch has fewer than 2^32 threads: a workgroup for every four of a row's pieces at most, 1,024 threads to finish it
+  const int64_t row_threads = std::max<int64_t>(kPartThreads * ((pieces + 3) / 4), 1024);
+  const int64_t group = std::min<int64_t>(filters ? p.group : B, 0xffffffffLL / row_threads);
   for (int64_t row0 = 0; row0 < B; row0 += group) {
     const int64_t rows = row0 + group < B ? group : B - row0;
     // a piece for each wave, or two where that makes more than enough workgroups
-    const int pieces = (int)((A + piece_length<T>() - 1) / piece_length<T>());
     const int per = rows * pieces >= 65536 ? 8 : 4;
     const int groups = (int)(rows * ((pieces + per - 1) / per));
     sample_maxima_kernel<T><<<groups, kPartThreads, 0, s>>>(logits, stride, (int)A, p, row0, per);
@@ -1348,8 +1351,8 @@ PARLHIP_EXPORT int parlhip_logits_sample(const void* logits, int dtype, int64_t 
                                          void* workspace, size_t workspace_bytes, parlhip_stream_t stream) {
   if (B < 0 || A < 1 || row_stride < A) return PARLHIP_EINVAL;
   if (dtype != PARLHIP_F32 && dtype != PARLHIP_BF16 && dtype != PARLHIP_F16) return PARLHIP_ENOSUP;
-  // one launch's threads: 64 for a row at most, or 256 for every eight of its 1,024 pieces
-  if (A > kSampleMaxActions || B > 0xffffffffLL / (A <= kWaveRow ? 64 : 256 * 128)) return PARLHIP_ENOSUP;
+  // up to 4,096 actions one launch of fewer than 2^32 threads: 64 for a row, four rows to a workgroup
+  if (A > kSampleMaxActions || B > (A <= kWaveRow ? ((int64_t)1 << 26) - 4 : ((int64_t)1 << 40) / A)) return PARLHIP_ENOSUP;
   if (!temperature && !(temperature_all >= 0.f && temperature_all < INFINITY)) return PARLHIP_EINVAL;
   if (!top_p && !(top_p_all >= 0.f)) return PARLHIP_EINVAL;
   if (!min_p && !(min_p_all >= 0.f && min_p_all <= 1.f)) return PARLHIP_EINVAL;

@@ -664,3 +664,17 @@ def test_a_filter_that_keeps_everything_changes_nothing(A, dtype, dev):
     for y, kw in ((x, dict(top_k=A)), (x, dict(top_k=k)), (x, dict(min_p=2.0**-44)), (x.float(), dict()), (x.float(), dict(top_k=A))):
         b, lq = ops.logits_sample(y, u, temperature=0.8, **kw)
         assert torch.equal(a, b) and torch.equal(lp, lq), kw
+
+
+@pytest.mark.parametrize('times', [190, 6000])
+def test_draw_from_any_number_of_long_rows(times, dev):
+    """133,000 rows, and more than four million (34 GB): each block of 700 is drawn as it is alone"""
+    from parl_amd import ops
+    A = 4097
+    block = _logits(700, A, torch.bfloat16, dev, 1)
+    u = torch.rand(700, generator=torch.Generator(device=dev).manual_seed(4), dtype=torch.float64, device=dev)
+    x, us = block.repeat(times, 1), u.repeat(times)
+    for s in (dict(), dict(temperature=0.0), dict(top_p=0.7)):
+        a, lp = ops.logits_sample(block, u, **s)
+        b, lq = ops.logits_sample(x, us, **s)
+        assert (b.view(times, 700) == a).all() and (lq.view(times, 700) == lp).all(), s

@@ -141,3 +141,16 @@ def test_host_tensors_are_refused(lib):
         ops.clip_grad_norm_([p], 1.0)
     with pytest.raises(ParlHipError):
         ops.grad_norm([p.grad])
+
+
+def test_rows_that_a_draw_takes(lib):
+    """what a launch of at most 2^32 - 1 threads takes, a wave for each row, up to 4,096 actions; above, launches follow each other"""
+    n = lambda B, A: _sample(lib, logits=None, B=B, A=A, stride=A)  # noqa: E731
+    for A in (1, 64, 65, 512, 513, 4096):
+        assert n((1 << 26) - 4, A) == INVALID          # the NULL pointer
+        for over in (3, 2, 1):
+            assert n((1 << 26) - over, A) == NOSUP     # four rows to a workgroup, rounded up
+    for A in (4097, 5000, 131072, 1 << 20):
+        assert n((1 << 40) // A, A) == INVALID
+        assert n((1 << 40) // A + 1, A) == NOSUP
+    assert n(131072, 5000) == n(200000, 5000) == INVALID
