@@ -12,7 +12,9 @@ entropies and their gradient (`ops.logits_log_prob`), the draw (`ops.logits_samp
 the clipping of the global gradient norm (`ops.clip_grad_norm_`) are the library's kernels instead of torch's
 Categorical and clip_grad_norm_, which materialise several arrays of the logits' size.  The policy may return float32,
 bfloat16 or float16 logits, and an action of -1 marks a row that is no decision: log-probability and entropy 0,
-no gradient from either."""
+no gradient from either.  sample() and predict() give it to a row whose every logit is -inf.  A row with NaN or +inf is a
+ValueError in sample(), predict() and learn(), as NaN is in Categorical; a call that is being captured into a graph
+cannot look at its results, there the row gets action -1 and, from sample(), NaN for log-probability and entropy."""
 import torch
 import torch.nn as nn
 from torch.distributions import Categorical, Normal
@@ -70,10 +72,22 @@ class PPO(Algorithm):
             return Normal(mean, std)
         return Categorical(logits=self.model.policy(obs))
 
+    @staticmethod
+    def _refuse(rows, what):
+        """ValueError where `rows` holds anywhere (waits for the device, as Categorical's own checks do).  False if the
+        call is being captured, so that nothing can be known."""
+        if torch.cuda.is_current_stream_capturing():
+            return False
+        n = int(rows.sum())
+        if n:
+            raise ValueError('PPO(fused_policy=True): %s in %d of %d rows' % (what, n, rows.numel()))
+        return True
+
     def _losses(self, obs, action, old_value, ret, old_logp, adv):
         """the three terms of the PPO objective for one minibatch (ppo.py:104-148)"""
         if self.fused_policy:
             logp, entropy = ops.logits_log_prob(self.model.policy(obs), action.to(torch.int64))
+            self._refuse(torch.isnan(logp), 'the policy has logits with NaN or +inf')
         else:
             dist = self._dist(obs)
             logp, entropy = dist.log_prob(action), dist.entropy()
@@ -117,8 +131,11 @@ class PPO(Algorithm):
         if self.fused_policy:
             logits = self.model.policy(obs)
             uniforms = torch.rand(logits.shape[:-1], dtype=torch.float64, device=logits.device)
-            action, _ = ops.logits_sample(logits, uniforms)
-            log_probs, entropy = ops.logits_log_prob(logits, action)
+            action, drawn = ops.logits_sample(logits, uniforms)
+            log_probs, entropy = ops.logits_log_prob(logits, action)   # the learner's own: its first ratio is 1
+            diverged = torch.isnan(drawn)
+            if not self._refuse(diverged, 'the policy has logits with NaN or +inf'):
+                log_probs, entropy = (t.masked_fill(diverged, float('nan')) for t in (log_probs, entropy))
             return value, action, log_probs, entropy
         dist = self._dist(obs)
         action = dist.sample()
@@ -133,7 +150,11 @@ class PPO(Algorithm):
             action, _ = self.model.policy(obs)
             return action
         if self.fused_policy:
-            return self.model.policy(obs).argmax(dim=-1, keepdim=True)
+            logits = self.model.policy(obs)
+            best = logits.amax(dim=-1, keepdim=True)
+            self._refuse(~(best < float('inf')), 'the policy has logits with NaN or +inf')
+            legal = (best > float('-inf')) & (best < float('inf'))
+            return logits.argmax(dim=-1, keepdim=True).masked_fill(~legal, -1)
         return Categorical(logits=self.model.policy(obs)).probs.argmax(dim=-1, keepdim=True)
 
     @torch.no_grad()

@@ -913,8 +913,9 @@ def ppo_sample_batch(obs, actions, logprobs, advantages, returns, values, idx):
 
 def logits_sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draw one action per row of logits [..., A] (float32 / bfloat16 / float16, A up to 2^20; up to 2^26 - 4 rows of at most
-    4,096 actions, above as many as there are) with the given uniforms (float64 [...], in [0, 1)): np.random.choice(A, 1, p=softmax(logits)) (examples/IMPALA/atari_agent.py:38-40) with the
-    usual filters, for action sets of any size.  Returns (actions int64 [...], log_probs float32 [...]).
+    4,096 actions, above as many as there are) with the given uniforms (float64 [...], in [0, 1)):
+    np.random.choice(A, 1, p=softmax(logits)) (examples/IMPALA/atari_agent.py:38-40) with the usual filters, for action sets
+    of any size.  Returns (actions int64 [...], log_probs float32 [...]).
 
     In the order (logit descending, index ascending) the longest prefix is kept whose actions have position < top_k, mass
     before them < top_p * mass of the top_k, and probability >= min_p * the largest; the first one always stays.  -inf

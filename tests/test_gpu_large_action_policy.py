@@ -179,3 +179,101 @@ def test_ppo_refuses_a_fused_policy_over_continuous_actions():
 
     with pytest.raises(AssertionError):
         PPO(Model(3, 4), continuous_action=True, fused_policy=True)
+
+
+def _table_ppo(logits, values, fused, **kw):
+    """PPO over a table: state s has the logits logits[s] and the value values[s]"""
+    from parl_amd.algorithms import PPO
+    import parl_amd as parl
+
+    class Model(parl.Model):
+        def __init__(self):
+            super().__init__()
+            self.logits = nn.Parameter(logits.clone())
+            self.values = nn.Parameter(values.clone())
+
+        def policy(self, obs):
+            return self.logits[obs]
+
+        def value(self, obs):
+            return self.values[obs].unsqueeze(-1)
+
+    args = dict(clip_param=0.2, value_loss_coef=0.5, entropy_coef=0.01, initial_lr=1e-2, eps=1e-5, max_grad_norm=0.2)
+    return PPO(Model(), fused_policy=fused, **dict(args, **kw))
+
+
+def _batch(alg, states, dev, seed=0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    obs = torch.arange(states, device=dev)
+    value, action, logp, _ = alg.sample(obs)
+    rand = lambda: torch.randn(states, generator=g, device=dev)  # noqa: E731
+    return [obs, action, value.view(-1) + rand(), rand(), logp + 0.1 * rand(), rand()]
+
+
+@pytest.mark.parametrize('A', [6, 700, 9000])
+def test_ppo_says_that_a_policy_has_diverged(A, dev):
+    """a row with NaN or +inf stops sample, predict and learn, as the NaN does without fused_policy; a row where nothing may be
+    taken is action -1 in sample and predict alike"""
+    from parl_amd import ops
+    logits = torch.randn(6, A, device=dev)
+    logits[1, A // 2] = float('nan')
+    logits[2] = float('nan')
+    logits[3, 0] = float('inf')
+    logits[4] = float('-inf')
+    alg, plain = (_table_ppo(logits, torch.zeros(6, device=dev), f) for f in (True, False))
+    at = lambda *s: torch.tensor(s, device=dev)  # noqa: E731
+    for s in (1, 2):
+        for a in (alg, plain):
+            with pytest.raises(ValueError):
+                a.sample(at(0, s))
+            with pytest.raises(ValueError):
+                a.predict(at(s, 0))
+    with pytest.raises(ValueError):
+        alg.sample(at(0, 3, 5))
+    with pytest.raises(ValueError):
+        alg.predict(at(0, 3, 5))
+    value, action, logp, entropy = alg.sample(at(0, 4, 5))
+    assert int(action[1]) == -1 and float(logp[1]) == 0 and float(entropy[1]) == 0
+    assert int(action[0]) >= 0 and int(action[2]) >= 0 and torch.isfinite(logp).all() and torch.isfinite(entropy).all()
+    best = alg.predict(at(0, 4, 5))
+    assert best.shape == (3, 1) and best.dtype == torch.int64
+    assert best.view(-1).tolist() == [int(logits[0].argmax()), -1, int(logits[5].argmax())]
+    z = torch.zeros(2, device=dev)
+    for s in (1, 2, 3):
+        before = [p.detach().clone() for p in alg.model.parameters()]
+        with pytest.raises(ValueError):
+            alg.learn(at(0, s), at(0, 1), z, z, z, torch.tensor([1.0, -1.0], device=dev))
+        for p, b in zip(alg.model.parameters(), before):
+            assert p.grad is None and torch.equal(p.detach().nan_to_num(7.0), b.nan_to_num(7.0))
+    # a row of padding is not looked at, whatever it holds
+    losses = alg.learn(at(0, 5, 1, 3), at(0, 1, -1, -1), *torch.zeros(3, 4, device=dev),
+                       torch.tensor([1.0, -1.0, 0.0, 0.0], device=dev))
+    assert all(math.isfinite(v) for v in losses)
+    assert torch.isfinite(alg.model.logits[0]).all() and torch.isfinite(alg.model.values).all()
+    assert ops.consume_device_errors() > 0   # the draws' flag is up as well
+
+
+def test_ppo_sample_in_a_graph_marks_what_it_cannot_raise(dev):
+    """a captured call cannot look at its results: the row of a diverged policy has no log-probability and no entropy"""
+    from parl_amd import ops
+    logits = torch.randn(4, 300, device=dev)
+    alg = _table_ppo(logits, torch.zeros(4, device=dev), True)
+    obs = torch.arange(4, device=dev)
+    alg.sample(obs)
+    alg.predict(obs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _, action, logp, entropy = alg.sample(obs)
+        best = alg.predict(obs)
+    for bad in (False, True, False):
+        with torch.no_grad():
+            alg.model.logits.copy_(logits)
+            if bad:
+                alg.model.logits[2, 7] = float('nan')
+        graph.replay()
+        torch.cuda.synchronize()
+        row = torch.tensor([False, False, bad, False], device=dev)
+        assert torch.equal(torch.isnan(logp), row) and torch.equal(torch.isnan(entropy), row)
+        assert torch.equal(action == -1, row) and torch.equal(best.view(-1) == -1, row)
+    assert ops.consume_device_errors() > 0
