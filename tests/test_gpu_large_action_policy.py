@@ -277,3 +277,21 @@ def test_ppo_sample_in_a_graph_marks_what_it_cannot_raise(dev):
         assert torch.equal(torch.isnan(logp), row) and torch.equal(torch.isnan(entropy), row)
         assert torch.equal(action == -1, row) and torch.equal(best.view(-1) == -1, row)
     assert ops.consume_device_errors() > 0
+
+
+@pytest.mark.parametrize('fused', [True, False])
+@pytest.mark.parametrize('A', [6, 700, 9000])
+def test_ppo_moves_every_parameter_by_its_clipped_gradient(A, fused, dev):
+    """Adam's first step from the gradients that learn() leaves: lr g / (|g| + eps)"""
+    alg = _table_ppo(torch.randn(20, A, device=dev), torch.randn(20, device=dev), fused)
+    batch = _batch(alg, 20, dev)
+    before = [p.detach().double().clone() for p in alg.model.parameters()]
+    alg.learn(*batch)
+    for p, b in zip(alg.model.parameters(), before):
+        g = p.grad.double()
+        step = 1e-2 * g / (g.abs() + 1e-5)
+        # float32: the parameter's own rounding, and a few roundings of the step (the square root of g^2 and its sum with
+        # eps, the two bias corrections); squares under the normal range leave a gradient of less than 1e-19 without effect
+        tol = 2.0**-23 * b.abs() + 2.0**-18 * step.abs() + 1e-2 * 1e-19 / 1e-5
+        assert ((p.double() - b + step).abs() <= tol).all()
+        assert (p.double() - b).abs().max() > 1e-3
