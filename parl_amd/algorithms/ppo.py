@@ -14,7 +14,8 @@ Categorical and clip_grad_norm_, which materialise several arrays of the logits'
 bfloat16 or float16 logits, and an action of -1 marks a row that is no decision: log-probability and entropy 0,
 no gradient from either.  sample() and predict() give it to a row whose every logit is -inf.  A row with NaN or +inf is a
 ValueError in sample(), predict() and learn(), as NaN is in Categorical; a call that is being captured into a graph
-cannot look at its results, there the row gets action -1 and, from sample(), NaN for log-probability and entropy."""
+cannot look at its results, there the row gets action -1 and, from sample(), NaN for log-probability and entropy.
+An action that is neither -1 nor one of the set is a ValueError in learn()."""
 import torch
 import torch.nn as nn
 from torch.distributions import Categorical, Normal
@@ -86,7 +87,9 @@ class PPO(Algorithm):
     def _losses(self, obs, action, old_value, ret, old_logp, adv):
         """the three terms of the PPO objective for one minibatch (ppo.py:104-148)"""
         if self.fused_policy:
-            logp, entropy = ops.logits_log_prob(self.model.policy(obs), action.to(torch.int64))
+            logits, taken = self.model.policy(obs), action.to(torch.int64)
+            self._refuse((taken < -1) | (taken >= logits.shape[-1]) | (taken != action), 'actions that are none')
+            logp, entropy = ops.logits_log_prob(logits, taken)
             self._refuse(torch.isnan(logp), 'the policy has logits with NaN or +inf')
         else:
             dist = self._dist(obs)

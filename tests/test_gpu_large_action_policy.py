@@ -295,3 +295,23 @@ def test_ppo_moves_every_parameter_by_its_clipped_gradient(A, fused, dev):
         tol = 2.0**-23 * b.abs() + 2.0**-18 * step.abs() + 1e-2 * 1e-19 / 1e-5
         assert ((p.double() - b + step).abs() <= tol).all()
         assert (p.double() - b).abs().max() > 1e-3
+
+
+@pytest.mark.parametrize('A', [6, 700, 9000])
+def test_ppo_refuses_actions_outside_the_set(A, dev):
+    from parl_amd import ops
+    ops.consume_device_errors()
+    alg, plain = (_table_ppo(torch.randn(4, A, device=dev), torch.zeros(4, device=dev), f) for f in (True, False))
+    before = [p.detach().clone() for p in alg.model.parameters()]
+    z, adv = torch.zeros(2, device=dev), torch.tensor([1.0, -1.0], device=dev)
+    for bad in (A, A + 5, -2):
+        for a in (alg, plain):
+            with pytest.raises(ValueError):
+                a.learn(torch.tensor([0, 1], device=dev), torch.tensor([0, bad], device=dev), z, z, z, adv)
+    for a in (alg, plain):
+        with pytest.raises(ValueError):
+            a.learn(torch.tensor([0, 1], device=dev), torch.tensor([0.0, 1.5], device=dev), z, z, z, adv)
+    for p, b in zip(alg.model.parameters(), before):
+        assert p.grad is None and torch.equal(p, b)
+    alg.learn(torch.tensor([0, 1], device=dev), torch.tensor([0.0, 2.0], device=dev), z, z, z, adv)   # whole numbers in any type
+    assert ops.consume_device_errors() == 0   # refused before any kernel saw them
