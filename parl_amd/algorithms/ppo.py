@@ -11,8 +11,9 @@ gather that feed learn() live in parl_amd.storage.RolloutStorage.
 entropies and their gradient (`ops.logits_log_prob`), the draw (`ops.logits_sample`, with uniforms of torch's generator) and
 the clipping of the global gradient norm (`ops.clip_grad_norm_`) are the library's kernels instead of torch's
 Categorical and clip_grad_norm_, which materialise several arrays of the logits' size.  The policy may return float32,
-bfloat16 or float16 logits, and an action of -1 marks a row that is no decision: log-probability and entropy 0,
-no gradient from either.  sample() and predict() give it to a row whose every logit is -inf.  A row with NaN or +inf is a
+bfloat16 or float16 logits, and an action of -1 marks a row that is no decision: sample() gives it log-probability and
+entropy 0, learn() takes its losses, their means and the advantages' normalisation over the other rows alone (one such row
+counts with the advantage 0, none with losses of 0).  sample() and predict() give it to a row whose every logit is -inf.  A row with NaN or +inf is a
 ValueError in sample(), predict() and learn(), as NaN is in Categorical; a call that is being captured into a graph
 cannot look at its results, there the row gets action -1 and, from sample(), NaN for log-probability and entropy.
 An action that is neither -1 nor one of the set is a ValueError in learn()."""
@@ -74,40 +75,61 @@ class PPO(Algorithm):
         return Categorical(logits=self.model.policy(obs))
 
     @staticmethod
-    def _refuse(rows, what):
-        """ValueError where `rows` holds anywhere (waits for the device, as Categorical's own checks do).  False if the
-        call is being captured, so that nothing can be known."""
+    def _refuse(bad, rows, what='the policy has logits with NaN or +inf'):
+        if bad:
+            raise ValueError('PPO(fused_policy=True): %s in %d of %d rows' % (what, bad, rows))
+
+    def _refuse_diverged(self, bad):
+        """ValueError where `bad` holds anywhere (waits for the device, as Categorical's own checks do).  False if the call is
+        being captured, so that nothing can be known."""
         if torch.cuda.is_current_stream_capturing():
             return False
-        n = int(rows.sum())
-        if n:
-            raise ValueError('PPO(fused_policy=True): %s in %d of %d rows' % (what, n, rows.numel()))
+        self._refuse(int(bad.sum()), bad.numel())
         return True
+
+    def _fused_log_prob(self, obs, action):
+        """log-probabilities and entropies, and the rows that are decisions (None: all are)"""
+        logits, taken = self.model.policy(obs), action.to(torch.int64)
+        outside = (taken < -1) | (taken >= logits.shape[-1]) | (taken != action)
+        taken = taken.masked_fill(outside, -1)
+        logp, entropy = ops.logits_log_prob(logits, taken)
+        live = (taken >= 0).view(-1)
+        n_outside, n_nan, n_live = torch.stack((outside.sum(), torch.isnan(logp).sum(), live.sum())).tolist()
+        self._refuse(n_outside, live.numel(), 'actions that are none')
+        self._refuse(n_nan, live.numel())
+        return logp, entropy, None if n_live == live.numel() else live.nonzero().view(-1)
 
     def _losses(self, obs, action, old_value, ret, old_logp, adv):
         """the three terms of the PPO objective for one minibatch (ppo.py:104-148)"""
+        rows = None   # where not all are decisions: those that are
         if self.fused_policy:
-            logits, taken = self.model.policy(obs), action.to(torch.int64)
-            self._refuse((taken < -1) | (taken >= logits.shape[-1]) | (taken != action), 'actions that are none')
-            logp, entropy = ops.logits_log_prob(logits, taken)
-            self._refuse(torch.isnan(logp), 'the policy has logits with NaN or +inf')
+            logp, entropy, rows = self._fused_log_prob(obs, action)
+            if rows is not None:
+                logp, entropy, old_value, ret, old_logp, adv = (t.reshape(-1)[rows]
+                                                                for t in (logp, entropy, old_value, ret, old_logp, adv))
         else:
             dist = self._dist(obs)
             logp, entropy = dist.log_prob(action), dist.entropy()
         if self.continuous_action:  # independent Normal per action dimension
             logp, entropy = logp.sum(1), entropy.sum(1)
         if self.norm_adv:  # ppo.py:124-127 on the device kernel (unbiased std, + 1e-8); no gradient
-            adv = ops.adv_normalize(adv.detach(), eps=1e-8).view_as(adv)
+            if self.fused_policy and adv.numel() == 1:   # it is its own mean, and there is no deviation
+                adv = torch.zeros_like(adv)
+            else:
+                adv = ops.adv_normalize(adv.detach(), eps=1e-8).view_as(adv)
+        mean = torch.sum if self.fused_policy and not adv.numel() else torch.mean   # of no decisions: 0
         eps = self.clip_param
         ratio = torch.exp(logp - old_logp)
-        policy_loss = -torch.minimum(ratio * adv, ratio.clamp(1.0 - eps, 1.0 + eps) * adv).mean()
+        policy_loss = -mean(torch.minimum(ratio * adv, ratio.clamp(1.0 - eps, 1.0 + eps) * adv))
         value = self.model.value(obs).view(-1)
+        if rows is not None:
+            value = value[rows]
         if self.use_clipped_value_loss:
             clipped = old_value + (value - old_value).clamp(-eps, eps)
-            value_loss = 0.5 * torch.maximum((value - ret)**2, (clipped - ret)**2).mean()
+            value_loss = 0.5 * mean(torch.maximum((value - ret)**2, (clipped - ret)**2))
         else:
-            value_loss = 0.5 * ((ret - value)**2).mean()
-        return value_loss, policy_loss, entropy.mean()
+            value_loss = 0.5 * mean((ret - value)**2)
+        return value_loss, policy_loss, mean(entropy)
 
     def learn(self, batch_obs, batch_action, batch_value, batch_return, batch_logprob, batch_adv, lr=None):
         """ppo.py:81-158: one clipped-surrogate update on a minibatch.  Returns
@@ -137,7 +159,7 @@ class PPO(Algorithm):
             action, drawn = ops.logits_sample(logits, uniforms)
             log_probs, entropy = ops.logits_log_prob(logits, action)   # the learner's own: its first ratio is 1
             diverged = torch.isnan(drawn)
-            if not self._refuse(diverged, 'the policy has logits with NaN or +inf'):
+            if not self._refuse_diverged(diverged):
                 log_probs, entropy = (t.masked_fill(diverged, float('nan')) for t in (log_probs, entropy))
             return value, action, log_probs, entropy
         dist = self._dist(obs)
@@ -155,7 +177,7 @@ class PPO(Algorithm):
         if self.fused_policy:
             logits = self.model.policy(obs)
             best = logits.amax(dim=-1, keepdim=True)
-            self._refuse(~(best < float('inf')), 'the policy has logits with NaN or +inf')
+            self._refuse_diverged(~(best < float('inf')))
             legal = (best > float('-inf')) & (best < float('inf'))
             return logits.argmax(dim=-1, keepdim=True).masked_fill(~legal, -1)
         return Categorical(logits=self.model.policy(obs)).probs.argmax(dim=-1, keepdim=True)

@@ -253,6 +253,72 @@ def test_ppo_says_that_a_policy_has_diverged(A, dev):
     assert ops.consume_device_errors() > 0   # the draws' flag is up as well
 
 
+@pytest.mark.parametrize('A', [6, 700, 9000])
+def test_ppo_refuses_actions_outside_the_set(A, dev):
+    from parl_amd import ops
+    ops.consume_device_errors()
+    alg, plain = (_table_ppo(torch.randn(4, A, device=dev), torch.zeros(4, device=dev), f) for f in (True, False))
+    before = [p.detach().clone() for p in alg.model.parameters()]
+    z, adv = torch.zeros(2, device=dev), torch.tensor([1.0, -1.0], device=dev)
+    for bad in (A, A + 5, -2):
+        for a in (alg, plain):
+            with pytest.raises(ValueError):
+                a.learn(torch.tensor([0, 1], device=dev), torch.tensor([0, bad], device=dev), z, z, z, adv)
+    for a in (alg, plain):
+        with pytest.raises(ValueError):
+            a.learn(torch.tensor([0, 1], device=dev), torch.tensor([0.0, 1.5], device=dev), z, z, z, adv)
+    for p, b in zip(alg.model.parameters(), before):
+        assert p.grad is None and torch.equal(p, b)
+    alg.learn(torch.tensor([0, 1], device=dev), torch.tensor([0.0, 2.0], device=dev), z, z, z, adv)   # whole numbers in any type
+    assert ops.consume_device_errors() == 0   # refused before any kernel saw them
+
+
+@pytest.mark.parametrize('norm_adv', [True, False])
+@pytest.mark.parametrize('clipped', [True, False])
+@pytest.mark.parametrize('A', [6, 700])
+def test_rows_of_action_minus_one_change_no_update(A, clipped, norm_adv, dev):
+    """a batch, and the same one with rows of padding between whose returns, advantages and old values are anything: the same
+    losses, gradients and parameters"""
+    g = torch.Generator(device=dev).manual_seed(A)
+    logits, values = torch.randn(40, A, generator=g, device=dev), torch.randn(40, generator=g, device=dev)
+    one, two = (_table_ppo(logits, values, True, use_clipped_value_loss=clipped, norm_adv=norm_adv) for _ in range(2))
+    batch = _batch(one, 24, dev)
+    at = torch.arange(24, device=dev) + torch.arange(24, device=dev) // 2   # every third row is padding
+    padded = []
+    for i, t in enumerate(batch):
+        p = torch.full((36, ), [30, -1, float('nan'), 1e30, float('nan'), float('-inf')][i], dtype=t.dtype, device=dev)
+        p[at] = t
+        padded.append(p)
+    for _ in range(2):
+        a, b = one.learn(*batch), two.learn(*padded)
+        # the same numbers through the same operations, but for the order of sums over 24 rows
+        assert a == pytest.approx(b, rel=24 * 2.0**-23, abs=24 * 2.0**-23)
+        for p, q in zip(one.model.parameters(), two.model.parameters()):
+            # one row of the batch for each row of the tables: a few products, the norm's factor
+            torch.testing.assert_close(p.grad, q.grad, rtol=2.0**-19, atol=1e-12)
+            torch.testing.assert_close(p, q, rtol=2.0**-20, atol=1e-2 * 2.0**-15)
+        assert (two.model.logits.grad[30] == 0).all() and float(two.model.values.grad[30]) == 0
+
+
+def test_a_batch_of_nothing_but_padding_teaches_nothing(dev):
+    alg = _table_ppo(torch.randn(4, 9, device=dev), torch.zeros(4, device=dev), True)
+    obs, none = torch.arange(4, device=dev), torch.full((4, ), -1, device=dev)
+    x = torch.full((4, ), float('nan'), device=dev)
+    assert alg.learn(obs, none, x, x, x, x) == (0.0, 0.0, 0.0)
+    for p in alg.model.parameters():
+        assert (p.grad == 0).all() and torch.isfinite(p).all()
+
+
+def test_one_decision_among_padding_is_learnt_from(dev):
+    """one advantage has no deviation to be divided by: it is its own mean, so it counts as 0 there"""
+    alg = _table_ppo(torch.randn(4, 9, device=dev), torch.zeros(4, device=dev), True)
+    obs, a = torch.arange(4, device=dev), torch.tensor([-1, 3, -1, -1], device=dev)
+    z = torch.zeros(4, device=dev)
+    losses = alg.learn(obs, a, z, z + 1, z, z + 5)
+    assert all(math.isfinite(v) for v in losses) and losses[0] == pytest.approx(0.5) and losses[1] == 0
+    assert float(alg.model.values[1]) != 0 and all(torch.isfinite(p).all() for p in alg.model.parameters())
+
+
 def test_ppo_sample_in_a_graph_marks_what_it_cannot_raise(dev):
     """a captured call cannot look at its results: the row of a diverged policy has no log-probability and no entropy"""
     from parl_amd import ops
@@ -295,23 +361,3 @@ def test_ppo_moves_every_parameter_by_its_clipped_gradient(A, fused, dev):
         tol = 2.0**-23 * b.abs() + 2.0**-18 * step.abs() + 1e-2 * 1e-19 / 1e-5
         assert ((p.double() - b + step).abs() <= tol).all()
         assert (p.double() - b).abs().max() > 1e-3
-
-
-@pytest.mark.parametrize('A', [6, 700, 9000])
-def test_ppo_refuses_actions_outside_the_set(A, dev):
-    from parl_amd import ops
-    ops.consume_device_errors()
-    alg, plain = (_table_ppo(torch.randn(4, A, device=dev), torch.zeros(4, device=dev), f) for f in (True, False))
-    before = [p.detach().clone() for p in alg.model.parameters()]
-    z, adv = torch.zeros(2, device=dev), torch.tensor([1.0, -1.0], device=dev)
-    for bad in (A, A + 5, -2):
-        for a in (alg, plain):
-            with pytest.raises(ValueError):
-                a.learn(torch.tensor([0, 1], device=dev), torch.tensor([0, bad], device=dev), z, z, z, adv)
-    for a in (alg, plain):
-        with pytest.raises(ValueError):
-            a.learn(torch.tensor([0, 1], device=dev), torch.tensor([0.0, 1.5], device=dev), z, z, z, adv)
-    for p, b in zip(alg.model.parameters(), before):
-        assert p.grad is None and torch.equal(p, b)
-    alg.learn(torch.tensor([0, 1], device=dev), torch.tensor([0.0, 2.0], device=dev), z, z, z, adv)   # whole numbers in any type
-    assert ops.consume_device_errors() == 0   # refused before any kernel saw them
