@@ -663,7 +663,7 @@ int parlhip_logits_log_prob_backward(const void* logits, int dtype, int64_t row_
  * grads = device pointers (dense memory, numel[i] elements of types[i]), numel, types.  Any number of tensors; empty ones
  * are skipped.  Squares and sums in float64, added in one fixed order (deterministic).  No host synchronisation;
  * capturable: the host arrays are read during the call only.  workspace: parlhip_grad_norm_workspace_bytes(...)
- * bytes, 8-byte aligned, for both entries.                                                                          */
+ * bytes, 8-byte aligned, for both entries.  PARLHIP_EINVAL where the workspace or norm_out overlaps a tensor or the other. */
 size_t parlhip_grad_norm_workspace_bytes(int n_tensors, const int64_t* numel);
 int parlhip_grad_norm(int n_tensors, const void* const* grads, const int64_t* numel, const int32_t* types,
                       void* workspace, size_t workspace_bytes, float* norm_out, parlhip_stream_t stream);

@@ -312,6 +312,21 @@ static int norm_overlap(int n_tensors, const void* const* grads, void* const* ou
   return rc;
 }
 
+// The partials and the norm overlap neither each other nor a tensor of the call.
+static bool norm_scratch_apart(int n_tensors, const void* const* grads, void* const* outs, const int64_t* numel,
+                               const int32_t* gt, const int32_t* ot, const void* workspace, size_t bytes, const float* norm_out) {
+  const auto meets = [](const void* a, size_t an, const void* b, size_t bn) {
+    return (uintptr_t)a < (uintptr_t)b + bn && (uintptr_t)b < (uintptr_t)a + an;
+  };
+  const auto hit = [&](const void* p, size_t n) { return meets(p, n, workspace, bytes) || meets(p, n, norm_out, sizeof(float)); };
+  if (meets(workspace, bytes, norm_out, sizeof(float))) return false;
+  for (int i = 0; i < n_tensors; ++i) {
+    if (numel[i] == 0) continue;
+    if (hit(grads[i], (size_t)numel[i] * type_size(gt[i])) || (outs && hit(outs[i], (size_t)numel[i] * type_size(ot[i])))) return false;
+  }
+  return true;
+}
+
 template <int READ, int WRITE>
 static int norm_launch(int n_tensors, const void* const* grads, void* const* outs, const int64_t* numel, const int32_t* gt,
                        const int32_t* ot, bool clip, double max_norm, double* partial, int n_partial, float* norm_out,
@@ -352,7 +367,9 @@ static int norm_run(int n_tensors, const void* const* grads, void* const* outs, 
   if (!norm_out) return PARLHIP_EINVAL;
   double* partial = (double*)workspace;
   if (!partial || (reinterpret_cast<uintptr_t>(partial) & 7)) return PARLHIP_EINVAL;
-  if (workspace_bytes < (size_t)(p > 0 ? p : 1) * sizeof(double)) return PARLHIP_ENOMEM;
+  const size_t bytes = (size_t)(p > 0 ? p : 1) * sizeof(double);
+  if (workspace_bytes < bytes) return PARLHIP_ENOMEM;
+  if (!norm_scratch_apart(n_tensors, grads, outs, numel, gt, ot, workspace, bytes, norm_out)) return PARLHIP_EINVAL;
   if (n_tensors <= kNormFew)
     return norm_launch<kNormFew, kNormFew>(n_tensors, grads, outs, numel, gt, ot, clip, max_norm, partial, (int)p, norm_out, s);
   return norm_launch<kNormRead, kNormWrite>(n_tensors, grads, outs, numel, gt, ot, clip, max_norm, partial, (int)p, norm_out, s);

@@ -154,3 +154,19 @@ def test_rows_that_a_draw_takes(lib):
         assert n((1 << 40) // A, A) == INVALID
         assert n((1 << 40) // A + 1, A) == NOSUP
     assert n(131072, 5000) == n(200000, 5000) == INVALID
+
+
+def test_scratch_memory_apart_from_the_tensors(lib):
+    """the partial sums and the norm are written while the gradients are still read"""
+    def arr(t, *v):
+        return (t * len(v))(*v)
+
+    P, I, T = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32
+    at, n, ty = arr(P, 4096, 8192), arr(I, 100, 200), arr(T, 0, 1)   # 4096..4495, 8192..8591
+    out = arr(P, 65536, 70000)                                       # 65536..65935, 70000..70399
+    for ws, norm in ((4096, 1024), (4488, 1024), (4088, 1024), (8584, 1024), (512, 4492), (512, 8192), (512, 512), (512, 524)):
+        assert lib.parlhip_grad_norm(2, at, n, ty, ws, 1 << 30, norm, None) == INVALID, (ws, norm)
+        assert lib.parlhip_clip_grad_norm(2, at, None, n, ty, None, 1.0, ws, 1 << 30, norm, None) == INVALID, (ws, norm)
+    for ws, norm in ((65536, 1024), (70392, 1024), (512, 65932), (512, 70396)):
+        assert lib.parlhip_clip_grad_norm(2, at, out, n, ty, ty, 1.0, ws, 1 << 30, norm, None) == INVALID, (ws, norm)
+    assert lib.parlhip_grad_norm(0, None, None, None, 512, 8, 516, None) == INVALID
