@@ -1,6 +1,7 @@
 """Hash of everything libparl_hip.so is built from: the hand-written sources, the public header, the
-cartridge translator and the cartridges it translates.  Used by the Makefile (baked into the library
-as parlhip_source_hash) and by tests/test_capi_symbols.py (recomputed from the tree)."""
+cartridge translator and the cartridges it translates; and one of what _torch_ops.so is.  Used by the Makefile (baked
+into the library as parlhip_source_hash, into the module as source_hash) and by tests/test_capi_symbols.py and
+tests/test_torch_ops_hash.py (recomputed from the tree)."""
 import glob
 import hashlib
 import os
@@ -21,9 +22,13 @@ def source_files():
     return sorted(fs)
 
 
-def source_hash():
+def torch_ops_files():
+    return [os.path.join(HERE, 'Makefile'), os.path.join(HERE, 'torch_ops.cpp'), os.path.join(ROOT, 'include', 'parl_hip.h')]
+
+
+def source_hash(files=None):
     h = hashlib.sha256()
-    for f in source_files():
+    for f in files or source_files():
         h.update(os.path.basename(f).encode() + b'\0')
         h.update(open(f, 'rb').read())
         h.update(b'\0')
@@ -32,5 +37,8 @@ def source_hash():
 
 if __name__ == '__main__':
     out = sys.argv[1]
+    if out == '--torch-ops':
+        print(source_hash(torch_ops_files()))
+        sys.exit()
     text = '#define PARLHIP_SOURCE_HASH "%s"\n' % source_hash()
     open(out, 'w').write(text)

@@ -375,6 +375,7 @@ py::object guarded(F f, const A&... a) {
 
 PYBIND11_MODULE(_torch_ops, m) {
   m.def("bind", &bind);
+  m.def("source_hash", [] { return PARL_SOURCE_HASH; });   // of what it was built from (srchash.py)
   m.def("logits_sample", [](py::handle a, py::handle b, py::handle c, py::handle d, py::handle e, py::handle f) {
     return guarded(logits_sample, a, b, c, d, e, f);
   });
