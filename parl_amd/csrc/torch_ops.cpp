@@ -4,7 +4,8 @@
 // costs tens of microseconds a call where there is an autograd node to build (a Python backward pass takes the
 // interpreter in the engine's thread) or a few hundred tensors to look at: more than the kernels behind it.  Here it is
 // C++: no computation, only the same checks and the same entries of libparl_hip.so, whose addresses bind() is given (so
-// that PARL_HIP_LIB goes for these too).  Every refusal is a ParlHipError.
+// that PARL_HIP_LIB goes for these too).  Every refusal of a call is a ParlHipError; what fails in a backward pass is the
+// RuntimeError that the autograd engine makes of it.
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <ATen/ops/zeros.h>
@@ -225,6 +226,8 @@ py::tuple logits_log_prob(const py::handle& logits_, const py::handle& actions_,
   const Tensor logits = unpack(logits_, "logits", name);
   check_logits(logits, name);
   const Tensor actions = per_row(unpack(actions_, "actions", name), at::kLong, logits, "actions", name);
+  if (THPVariable_Check(temperature.ptr()) && THPVariable_Unpack(temperature.ptr()).numel() != 1)
+    refuse(name, ": temperature must be one number for all rows; for one of each row's own divide the logits by it first");
   const double t = number(temperature, "temperature", name);
   if (!(t > 0.0) || std::isinf((float)t)) refuse(name, ": temperature must be a finite float32 > 0, got ", t);
   torch::autograd::variable_list out;

@@ -937,7 +937,11 @@ def logits_log_prob(logits, actions, temperature=1.0):
 
     Action -1 marks a row that is no decision (padding behind a sequence's end): log_prob 0, entropy 0, zero gradient; so
     does a row whose every logit is -inf.  Another index outside [0, A) is clamped and raises the flag of
-    consume_device_errors().  A row with NaN or +inf gives NaN; the other rows are not touched by it."""
+    consume_device_errors().  A row with NaN or +inf gives NaN; the other rows are not touched by it.
+
+    temperature is one number for all rows.  Rows drawn with temperatures of their own: logits / temperature.unsqueeze(-1), in
+    float32, and temperature 1.  The backward pass reads the logits and the returned entropies again: neither may be
+    changed in place before it (autograd says so)."""
     return N.torch_ops().logits_log_prob(logits, actions, temperature)
 
 
@@ -960,6 +964,7 @@ def clip_grad_norm_(parameters, max_norm, *, error_if_nonfinite=False, out=None)
 
 
 def consume_device_errors():
-    """Synchronise and return/clear the device-side data-error flag (bad action index)."""
+    """Synchronise and return/clear the current device's data-error flag (a bad action or minibatch index, a row of
+    logits_sample with NaN or +inf)."""
     return N.check(N.lib().parlhip_consume_device_errors(N.stream_ptr()),
                    'parlhip_consume_device_errors')

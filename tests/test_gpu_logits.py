@@ -678,3 +678,21 @@ def test_draw_from_any_number_of_long_rows(times, dev):
         a, lp = ops.logits_sample(block, u, **s)
         b, lq = ops.logits_sample(x, us, **s)
         assert (b.view(times, 700) == a).all() and (lq.view(times, 700) == lp).all(), s
+
+
+def test_log_prob_with_a_temperature_for_each_row(dev):
+    """is refused by its name; the logits divided by it are the same policy, which the draw's log_probs agree with"""
+    from parl_amd import ops
+    from parl_amd._native import ParlHipError
+    rows, A = 24, 5000
+    x = _logits(rows, A, torch.bfloat16, dev, 3)
+    g = torch.Generator(device=dev).manual_seed(1)
+    u, t = torch.rand(rows, generator=g, dtype=torch.float64, device=dev), torch.rand(rows, generator=g, device=dev) + 0.3
+    a, lp = ops.logits_sample(x, u, temperature=t)
+    with pytest.raises(ParlHipError, match='divide the logits'):
+        ops.logits_log_prob(x, a, temperature=t)
+    got, _ = ops.logits_log_prob(x.float() / t.unsqueeze(-1), a)
+    # float32 logits of up to 45, divided: half a step each of the row's largest and the action's; sums as in check_logp
+    torch.testing.assert_close(got, lp, rtol=2.0**-22, atol=2.0**-24 * (2 * 45 + (A / 256 + 32) * (math.log(A) + 1)))
+    one, _ = ops.logits_log_prob(x, a, temperature=torch.tensor(0.7))
+    assert torch.equal(one, ops.logits_log_prob(x, a, temperature=float(torch.tensor(0.7)))[0])
