@@ -648,6 +648,7 @@ int parlhip_logits_sample(const void* logits, int dtype, int64_t row_stride, con
  * (8-byte aligned, may be NULL): what the backward pass needs, the row's maximum and its sum of exp((x - max) / T).
  * Action -1 marks a row that is no decision (padding): 0, 0, and a zero gradient; so does a row whose every logit is -inf.
  * Another index outside [0,A) is clamped and raises the data-error flag.  A row with a NaN or +inf gives NaN.  float32 sums.
+ * A <= 2^31, N * A <= 2^40; above 512 actions a launch takes fewer than 2^32 threads, 64 to 1,024 for a row (else PARLHIP_ENOSUP).
  * workspace: parlhip_logits_log_prob_workspace_bytes(N, A) bytes (few long rows are split), 4-byte aligned.            */
 size_t parlhip_logits_log_prob_workspace_bytes(int64_t N, int64_t A);
 int parlhip_logits_log_prob(const void* logits, int dtype, int64_t row_stride, const int64_t* actions, float* log_probs,

@@ -8,9 +8,11 @@
 // the multiply-add hide behind the loads), one partial per workgroup, all partials added in one fixed order: the same
 // gradients give the same bits in every call.  The tensors' addresses travel as kernel arguments, so nothing is copied to
 // the device and a captured call carries its own table.
-// Measured: 1.1 G bf16 values in 435 tensors into bf16, read twice and written once (6.6 GB), 1,283 us = 5.1 TB/s (a large copy:
-// 4.9); 120 M into float32, whose second read the 256 MB cache serves, 231 us; the 42x42 model's ten float32 gradients
-// 9.5 us, two launches of 4.  Four workgroups per CU were 3 % slower than two over 2 GB, one 30 %.
+// Measured: 1.1 G bf16 values in 435 tensors into bf16, read twice and written once (6.6 GB), 1,284 us = 5.1 TB/s (a large copy:
+// 4.9); 120 M into float32 (240 MB read twice, 480 written) 232 us: two launches of 81 together for the norm, which alone,
+// call after call, takes 54, and two of 150 that move 4.8 TB/s; the 42x42 model's ten float32 gradients 9.3 us, two
+// launches of 4.  In place and under the bound the scaling launches still walk over their chunks: 1.1 G values 584 us, the
+// norm alone 428.  Four workgroups per CU were 3 % slower than two over 2 GB, one 30 %.
 #include "common.hpp"
 #include "logits_common.hpp"
 #include <algorithm>

@@ -7,9 +7,10 @@
 // Forward: one pass over the row with the running maximum m, s = sum e^{z-m} and t = sum e^{z-m} (z - m), all in float32 and
 // rescaled when m grows; H = log s - t / s.  The backward pass gets (m, s) and H, so it reads the row once and writes its
 // gradient once; the probabilities are never stored.  Both passes are bound by HBM: one exp and some ten float
-// operations per two or four bytes.  Rows whose action is -1 are not read.  4,096 x 131,072 bf16, a tenth of the rows ignored:
-// forward 0.97 GB in 217 us (4.5 TB/s), backward 2.0 GB in 368 us (5.5 TB/s); a large copy moves 4.9 TB/s here.  At
-// 51,200 x 6 each is a launch of 4 us, and the 54 us of a call are the autograd engine's.
+// operations per two or four bytes.  Rows of more than 512 actions whose action is -1 are not read (of fewer, all are: they
+// lie side by side).  4,096 x 131,072 bf16, a tenth of the rows ignored: 579 us for both passes; under the tracer, which
+// adds to them, forward 0.97 GB in 225 us (4.3 TB/s), backward 2.0 GB in 365 us (5.6 TB/s); a large copy moves 4.9 TB/s
+// here.  At 51,200 x 6 each is a launch of 4 us, and the rest of a call's 31 to 54 us are the autograd engine's.
 #include "common.hpp"
 #include "logits_common.hpp"
 

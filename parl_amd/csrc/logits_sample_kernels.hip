@@ -26,12 +26,14 @@
 // Rows of up to 4,096 actions do that in one wave each.  Above, every pass over the rows is a launch of its own over segments of
 // all rows, which fills the card whether the rows are many or few and long, and a workgroup per row finishes.
 //
-// Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 144 us, 55 us of which one read of
-// the 268 MB would take: 38 for the maxima (HBM and cache), 100 for the masses (the vector unit, 25 instructions a value), 8 for
-// the finish.  Sums relative to the pieces' own maxima, in one pass, took 110 and were another distribution (above).
-// 1,024 x 100,003 with top-p 0.95: 31 us for the maxima, 84 for the classes (24 instructions a value), 92 for the finish
-// (a pass over the row by each workgroup, and the chain of scans behind it), 212 with what lies between them.  One row of
-// 131,072 with top-k and top-p: 27 us, three launches of 4, 7 and 14, the last a chain of scans.
+// Measured (a large copy on this card moves 4.9 TB/s): 1,024 x 131,072 bf16 without filters 140 to 144 us, 55 us of which one
+// read of the 268 MB would take; under the tracer 40 for the maxima (HBM and cache), 102 for the masses (the vector unit, which
+// issues in 91 % of its slots, 25 instructions a value), 8 for the finish.  Sums relative to the pieces' own maxima, in one
+// pass, took 110 and were another distribution (above).  1,024 x 100,003 with top-p 0.95: 31 us for the maxima, 84 for the
+// classes (24 instructions a value), 93 for the finish (a pass over the row by each workgroup, and the chain of scans behind
+// it), 205 to 212 for the call.  One row of 131,072 with top-k and top-p: 26 us, three launches of 4, 7 and 14, the last a
+// chain of scans.  Values that lie close together meet in few classes: 1,024 x 131,072 with top-p 0.9 takes 217 us at a
+// spread of 2.5 and 625 at 0.3.
 #include "common.hpp"
 #include "logits_common.hpp"
 #include <algorithm>

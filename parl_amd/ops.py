@@ -955,7 +955,7 @@ def clip_grad_norm_(parameters, max_norm, *, error_if_nonfinite=False, out=None)
     """torch.nn.utils.clip_grad_norm_(parameters, max_norm) (parl/algorithms/torch/a2c.py:76-78) over any number of
     parameters whose gradients are float32 / bfloat16 / float16 (mixed): every .grad times min(1, max_norm / (norm + 1e-6)),
     in two launches for up to 168 gradients.  Returns the norm before clipping, a float32 scalar tensor on the device (no
-    synchronisation, unless error_if_nonfinite asks for one).
+    synchronisation, unless error_if_nonfinite asks for one; it also reads the gradients once more).
 
     out: a list of tensors, one for each parameter with a gradient, that receive the clipped gradients instead (of any
     of the three types, e.g. the float32 gradients of master weights); the .grad stay as they are.  A gradient
