@@ -105,8 +105,9 @@ class PPO(Algorithm):
         if self.fused_policy:
             logp, entropy, rows = self._fused_log_prob(obs, action)
             if rows is not None:
-                logp, entropy, old_value, ret, old_logp, adv = (t.reshape(-1)[rows]
-                                                                for t in (logp, entropy, old_value, ret, old_logp, adv))
+                logp, entropy, ret, old_logp, adv = (t.reshape(-1)[rows] for t in (logp, entropy, ret, old_logp, adv))
+                if self.use_clipped_value_loss:
+                    old_value = old_value.reshape(-1)[rows]
         else:
             dist = self._dist(obs)
             logp, entropy = dist.log_prob(action), dist.entropy()

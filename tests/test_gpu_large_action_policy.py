@@ -361,3 +361,10 @@ def test_ppo_moves_every_parameter_by_its_clipped_gradient(A, fused, dev):
         tol = 2.0**-23 * b.abs() + 2.0**-18 * step.abs() + 1e-2 * 1e-19 / 1e-5
         assert ((p.double() - b + step).abs() <= tol).all()
         assert (p.double() - b).abs().max() > 1e-3
+
+
+def test_old_values_that_no_loss_reads_may_be_missing(dev):
+    alg = _table_ppo(torch.randn(6, 9, device=dev), torch.zeros(6, device=dev), True, use_clipped_value_loss=False)
+    obs, action, _, ret, logp, adv = _batch(alg, 6, dev)
+    for a in (action, torch.where(obs == 3, -1, action)):
+        assert all(math.isfinite(v) for v in alg.learn(obs, a, None, ret, logp, adv))
