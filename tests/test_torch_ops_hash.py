@@ -7,6 +7,9 @@ from conftest import ROOT
 
 def test_torch_ops_match_the_sources():
     from parl_amd import _native
+    if not os.path.exists(os.path.join(ROOT, 'parl_amd', '_torch_ops.so')):
+        import __graft_entry__
+        __graft_entry__.build()
     csrc = os.path.join(ROOT, 'parl_amd', 'csrc')
     sys.path.insert(0, csrc)
     try:
