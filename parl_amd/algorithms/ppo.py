@@ -93,7 +93,7 @@ class PPO(Algorithm):
         outside = (taken < -1) | (taken >= logits.shape[-1]) | (taken != action)
         taken = taken.masked_fill(outside, -1)
         logp, entropy = ops.logits_log_prob(logits, taken)
-        live = (taken >= 0).view(-1)
+        live = (taken >= 0).reshape(-1)
         n_outside, n_nan, n_live = torch.stack((outside.sum(), torch.isnan(logp).sum(), live.sum())).tolist()
         self._refuse(n_outside, live.numel(), 'actions that are none')
         self._refuse(n_nan, live.numel())
@@ -122,7 +122,7 @@ class PPO(Algorithm):
         eps = self.clip_param
         ratio = torch.exp(logp - old_logp)
         policy_loss = -mean(torch.minimum(ratio * adv, ratio.clamp(1.0 - eps, 1.0 + eps) * adv))
-        value = self.model.value(obs).view(-1)
+        value = self.model.value(obs).reshape(-1)
         if rows is not None:
             value = value[rows]
         if self.use_clipped_value_loss:

@@ -368,3 +368,15 @@ def test_old_values_that_no_loss_reads_may_be_missing(dev):
     obs, action, _, ret, logp, adv = _batch(alg, 6, dev)
     for a in (action, torch.where(obs == 3, -1, action)):
         assert all(math.isfinite(v) for v in alg.learn(obs, a, None, ret, logp, adv))
+
+
+def test_actions_in_any_memory_order(dev):
+    """a batch [T, B] that lies transposed, with padding: as the flat one"""
+    logits = torch.randn(12, 9, device=dev)
+    one, two = (_table_ppo(logits, torch.zeros(12, device=dev), True) for _ in range(2))
+    obs, action, value, ret, logp, adv = _batch(one, 12, dev)
+    action[5] = -1
+    flat = one.learn(obs, action, value, ret, logp, adv)
+    t = lambda x: x.view(3, 4).t().contiguous().t()  # noqa: E731
+    assert not t(action).is_contiguous()
+    assert two.learn(t(obs), t(action), t(value), t(ret), t(logp), t(adv)) == pytest.approx(flat, rel=12 * 2.0**-23)
